@@ -162,6 +162,55 @@ STTX_EXPORT int STTX_InferChunk(ModelState* aCtx, const float* aMfcc, unsigned i
                                const float* aStateH, float* aProbs, float* aNewStateC, float* aNewStateH);
 STTX_EXPORT int STTX_GetGeometry(const ModelState* aCtx, int* aOut10);
 
+/* ---- 8-bit floating point in blocks of 128 (device pointers, the caller's stream) ---------------
+ * The dense layers of this path in a third arithmetic beside f16 and the released models' int8 (STTX_GetAcousticMode): e4m3 values (4 exponent
+ * bits, 3 mantissa bits, largest 448, no infinity) with one power of two per block of 128 values along a row.
+ *
+ * A matrix IN BLOCKS of 1 x 128 (activations) or 128 x 128 (weights) is
+ *   values  e4m3 bytes [rows][ld]: a row holds its columns and zeros up to a multiple of 128; rows start at multiples of 16 bytes
+ *   scale   bytes [rows, or rows / 128 rounded up][ld_scale]: byte s of a block stands for 2^(s - 127); a row holds its blocks, padded to a
+ *           multiple of 4 (the entries below write 127 there); rows start at multiples of 4 bytes
+ *   value (r, c) = values[r][c] * 2^(scale[r or r / 128][c / 128] - 127); scale byte 255 makes its whole block NaN.
+ * Quantising: with t the largest finite |x| of a block, its power is the smallest 2^e >= 2^-127 with t <= 448 * 2^e (2^0 where t = 0); a value
+ * becomes the e4m3 nearest to x / 2^e, ties to even; infinities and NaN become NaN and do not move their block's power.  Reading back rounds
+ * once, to the type asked for.
+ *
+ * All pointers are device pointers; rows have unit column stride, row strides are in elements (bytes for values and scales).  A row stride of an
+ * input may be anything from 0 (every row the same one); an output's is at least its columns.  Zero rows are a call that does nothing.  Outputs
+ * must not overlap inputs or each other.  The calls enqueue on aStream (a hipStream_t of any device; NULL = the current device's null stream),
+ * allocate nothing, keep nothing and do not wait: they may be captured into a HIP graph, and called from several threads at once.
+ * STT_ERR_INVALID_SHAPE (a line on stderr says what): an argument is outside the above, nothing was enqueued. */
+enum STTX_ElementType { STTX_F32 = 0, STTX_F16 = 1, STTX_BF16 = 2, STTX_E4M3 = 3 };
+/* aX [aRows][aCols] of aType (STTX_F32, STTX_F16, STTX_BF16) -> aQ, aScale in blocks of aBlockRows (1 or 128) x 128.  With 1-row blocks up to
+ * 2^31 - 1 rows, with 128-row blocks up to 128 * 65535. */
+STTX_EXPORT int STTX_QuantizeBlocks(const void* aX, int aType, long long aRows, long long aCols, long long aLdX, int aBlockRows, unsigned char* aQ,
+                                   long long aLdQ, unsigned char* aScale, long long aLdScale, void* aStream);
+/* ... and back: aY [aRows][aCols] of aType. */
+STTX_EXPORT int STTX_DequantizeBlocks(const unsigned char* aQ, long long aLdQ, const unsigned char* aScale, long long aLdScale, long long aRows,
+                                     long long aCols, int aBlockRows, void* aY, int aType, long long aLdY, void* aStream);
+/* A dense layer: y[m][n] = epi(sum over k of x[m][k] * w[n][k] + bias[n]), sums in 32 bits; epi is nothing, or (relu_clip > 0) the graph's clipped
+ * ReLU min(max(y, 0), relu_clip) -- NaN stays NaN.  Operands count as float32 holds them: beyond its range (scale bytes above 247) they are
+ * infinities; magnitudes below 2^-126 may count as zero. */
+typedef struct STTX_DenseBlocksArgs {
+  const void* x;                    /* [rows][in]: in blocks of 1 x 128 (x_type STTX_E4M3, x_scale), or f32 / f16 / bf16, quantised so by the call */
+  const unsigned char* x_scale;
+  const unsigned char* w;           /* [out][in] in blocks of 128 x 128 */
+  const unsigned char* w_scale;
+  const float* bias;                /* [out], or NULL */
+  void* y;                          /* [rows][out]: f32 / f16 / bf16, or (y_type STTX_E4M3, y_scale) written in blocks of 1 x 128 for the next layer */
+  unsigned char* y_scale;
+  void* workspace;                  /* STTX_DenseBlocksWorkspace bytes at a multiple of 16, this call's own until it has run; may be NULL where 0 */
+  void* stream;
+  long long x_ld, x_scale_ld, w_ld, w_scale_ld, y_ld, y_scale_ld;
+  unsigned long long workspace_bytes;
+  long long rows, in, out;
+  int x_type, y_type;
+  float relu_clip;                  /* 0: no ReLU */
+} STTX_DenseBlocksArgs;
+STTX_EXPORT int STTX_DenseBlocks(const STTX_DenseBlocksArgs* aArgs);
+/* Bytes of workspace such a call needs (0 for x in blocks, and for few rows: those are quantised on the way into the product). */
+STTX_EXPORT unsigned long long STTX_DenseBlocksWorkspace(int aXType, long long aRows, long long aIn);
+
 /* ---- decoder on caller-supplied emissions ----------------------------------------------------- */
 typedef struct STTX_Decoder STTX_Decoder;
 /* aNumStreams independent DecoderStates sharing the model's alphabet, scorer and hot words (captured now).

@@ -134,6 +134,41 @@ struct SoftmaxArgs {
   int exact;            // int8 path: every probability the correctly rounded float of exp(l - max) / sum (float64 evaluation, one rounding each)
 };
 
+// ---- 8-bit floating point in blocks of 128 (kernels_blocks.hip: the format; include/stt_amd.h: STTX_QuantizeBlocks & co.)
+// A matrix in blocks: e4m3 values [rows][ld], ld a multiple of 16 and at least the columns rounded up to 128 (zeros there), 16-byte aligned; scale
+// bytes [rows, or rows / 128 rounded up][lds], lds a multiple of 4 and at least the blocks of a row rounded up to 4, 4-byte aligned.
+enum { BLOCKS_F32 = 0, BLOCKS_F16 = 1, BLOCKS_BF16 = 2, BLOCKS_E4M3 = 3 };
+struct BlocksQuantArgs {
+  const void* x;            // [rows][ldx] of `type`
+  unsigned char *q, *scale;
+  int64_t rows, ldx, ldq, lds;
+  int cols, type, block_rows;   // block_rows: 1 or 128
+  int vec;                  // rows of x may be read 16 bytes at a time
+};
+struct BlocksDequantArgs {
+  const unsigned char *q, *scale;
+  void* y;                  // [rows][ldy] of `type`
+  int64_t rows, ldq, lds, ldy;
+  int cols, type, block_rows;
+  int vec;                  // rows of y may be written 16 bytes at a time
+};
+struct BlocksDenseArgs {
+  const void* x;            // [M][ldx]: e4m3 in blocks of 1 x 128 with x_scale, or f32 / f16 / bf16 (blocks_dense_fused(M) only)
+  const unsigned char *x_scale, *w, *w_scale;   // w [N][ldw] in blocks of 128 x 128
+  const float* bias;        // [N] or null
+  void* y;                  // [M][ldy] f32 / f16 / bf16, or e4m3 in blocks of 1 x 128 with y_scale
+  unsigned char* y_scale;
+  int64_t M, ldx, ldxs, ldw, ldws, ldy, ldys;
+  int N, K, x_type, y_type, relu;
+  float clip;
+  int xvec;                 // rows of an f32 / f16 / bf16 x may be read 16 bytes at a time
+  int vec;                  // rows of y may be written four values at a time
+};
+void launch_blocks_quantize(const BlocksQuantArgs& a, hipStream_t st);
+void launch_blocks_dequantize(const BlocksDequantArgs& a, hipStream_t st);
+bool blocks_dense_fused(int64_t M);   // launch_blocks_dense quantises this many rows itself; more have to be in blocks already
+void launch_blocks_dense(const BlocksDenseArgs& a, hipStream_t st);
+
 // dst/src: device-addressable (HBM or mapped page-locked host memory); any size, any alignment
 void launch_copy_bytes(void* dst, const void* src, size_t bytes, hipStream_t st);
 void launch_placement_hog(unsigned* scratch, hipStream_t st);    // a dispatch that keeps its pipe for ~0.2 ms (engine.cpp: place_engine_streams)

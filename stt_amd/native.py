@@ -35,6 +35,12 @@ class ModelInfo(C.Structure):  # STTX_ModelInfo, include/stt_amd.h
                                                                       ("asymmetric_quantize_inputs", C.c_int)]
 
 
+class DenseBlocksArgs(C.Structure):  # STTX_DenseBlocksArgs, include/stt_amd.h
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "x_scale", "w", "w_scale", "bias", "y", "y_scale", "workspace", "stream")] +
+                [(n, C.c_longlong) for n in ("x_ld", "x_scale_ld", "w_ld", "w_scale_ld", "y_ld", "y_scale_ld")] + [("workspace_bytes", C.c_ulonglong)] +
+                [(n, C.c_longlong) for n in ("rows", "inner", "out")] + [("x_type", C.c_int), ("y_type", C.c_int), ("relu_clip", C.c_float)])
+
+
 class Metadata(C.Structure):
     _fields_ = [("transcripts", C.POINTER(CandidateTranscript)), ("num_transcripts", C.c_uint),
                 ("emissions", C.POINTER(AcousticModelEmissions))]
@@ -60,7 +66,7 @@ STT_AMD_H = [
     "STTX_DecoderCreate", "STTX_DecoderNext", "STTX_DecoderDecode", "STTX_DecoderBeam", "STTX_DecoderStats", "STTX_DecoderErrorBits",
     "STTX_DecoderSetProfiling", "STTX_DecoderGetProfile", "STTX_DecoderFree", "STTX_PackLstmRecurrent", "STTX_InspectModel", "STTX_ReadModelTensor",
     "STTX_FleetCreate", "STTX_FleetSize", "STTX_FleetEnableExternalScorer", "STTX_FleetSetBeamWidth", "STTX_FleetSpeechToTextBatch",
-    "STTX_FleetFree", "STTX_ShardUtterances",
+    "STTX_FleetFree", "STTX_ShardUtterances", "STTX_QuantizeBlocks", "STTX_DequantizeBlocks", "STTX_DenseBlocks", "STTX_DenseBlocksWorkspace",
 ]
 STT_AMD_TEST_H = [      # include/stt_amd_test.h: libstt_test.so only
     "STTX_DebugBatchProbs", "STTX_TestLstmSteps", "STTX_TestDenseHybrid", "STTX_DebugSlowRows", "STTX_TestHybridChain", "STTX_TestDense",
@@ -80,7 +86,7 @@ def lib():
                            "there is no fallback implementation." % LIB_PATH)
     L = C.CDLL(LIB_PATH)
     L.STTX_ConfigureRuntime()      # before the first HIP call of this process (include/stt_amd.h)
-    vp, ci, cu, cf, cd, cs = C.c_void_p, C.c_int, C.c_uint, C.c_float, C.c_double, C.c_char_p
+    vp, ci, cu, cf, cd, cs, cl = C.c_void_p, C.c_int, C.c_uint, C.c_float, C.c_double, C.c_char_p, C.c_longlong
     pp = C.POINTER
     sig = {
         "STT_CreateModel": (ci, [cs, pp(vp)]),
@@ -173,6 +179,10 @@ def lib():
         "STTX_FleetSpeechToTextBatch": (pp(vp), [vp, pp(vp), pp(cu), cu]),
         "STTX_FleetFree": (None, [vp]),
         "STTX_ShardUtterances": (ci, [pp(cu), cu, cu, pp(cu)]),
+        "STTX_QuantizeBlocks": (ci, [vp, ci, cl, cl, cl, ci, vp, cl, vp, cl, vp]),
+        "STTX_DequantizeBlocks": (ci, [vp, cl, vp, cl, cl, cl, ci, vp, ci, cl, vp]),
+        "STTX_DenseBlocks": (ci, [pp(DenseBlocksArgs)]),
+        "STTX_DenseBlocksWorkspace": (C.c_ulonglong, [ci, cl, cl]),
         "STTX_TestFleetRecords": (pp(vp), [pp(cs), pp(cu), cu, cu]),
         "STTX_DebugFleetFailShard": (ci, [vp, ci]),
     }
