@@ -8,6 +8,9 @@ tensors in HBM: 8-bit floating point (e4m3) with one power of two per block of 1
 
 Calls enqueue on torch's current stream of the tensors' device and allocate with torch, so they can be captured into a graph like any torch
 call.  No compute happens in Python; there is no fallback for tensors elsewhere.
+
+A call on a few rows is over in less time than a careless caller needs to make it, so the checks below are one expression each on the way that
+succeeds, and the messages are put together on the way that fails.
 """
 import ctypes as C
 
@@ -17,11 +20,19 @@ from . import native
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
-_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, E4M3: 3}   # STTX_ElementType
+_PLAIN = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}            # STTX_ElementType
+_E4M3 = 3
+_UINT8 = torch.uint8
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_lib = None
 
 
-def _up(n, to):
-    return -(-n // to) * to
+def _entry():
+    """The library and the number of devices, looked up on first use."""
+    global _lib, _devices
+    _devices = torch.cuda.device_count()
+    _lib = native.lib()
+    return _lib
 
 
 class BlockTensor(object):
@@ -40,74 +51,80 @@ class BlockTensor(object):
         return "BlockTensor(%d x %d, blocks of %d x %d)" % (self.values.shape[0], self.cols, self.block_rows, BLOCK)
 
 
-def _plain(t, what):
-    if t.dim() != 2 or t.dtype not in _TYPES or t.dtype is E4M3:
-        raise ValueError("%s: a two-dimensional float32, float16 or bfloat16 tensor is wanted, got %s %s" % (what, t.dtype, tuple(t.shape)))
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        raise ValueError("%s: columns have to be contiguous (stride 1), got stride %d" % (what, t.stride(1)))
+def _bad_plain(t, what):
+    if t.dim() != 2 or t.dtype not in _PLAIN:
+        return ValueError("%s: a two-dimensional float32, float16 or bfloat16 tensor is wanted, got %s %s" % (what, t.dtype, tuple(t.shape)))
+    if t.shape[1] < 1:
+        return ValueError("%s: at least one column is wanted" % what)
     if not t.is_cuda:
-        raise ValueError("%s: has to be in GPU memory, got a tensor on %s" % (what, t.device))
+        return ValueError("%s: has to be in GPU memory, got a tensor on %s" % (what, t.device))
+    return ValueError("%s: columns have to be contiguous (stride 1), got stride %d" % (what, t.stride(1)))
 
 
-def _blocks(b, what, block_rows=None):
+def _plain(t, what):
+    """(type, rows, cols, row stride, device index)"""
+    shape, kind = t.shape, _PLAIN.get(t.dtype, -1)
+    if kind < 0 or len(shape) != 2 or shape[1] < 1 or not t.is_cuda or (t.stride(1) != 1 and shape[1] > 1):
+        raise _bad_plain(t, what)
+    return kind, shape[0], shape[1], t.stride(0), t.get_device()
+
+
+def _bad_blocks(b, what, block_rows):
     v, s = b.values, b.scale
-    if v.dtype is not E4M3 or v.dim() != 2 or s.dtype is not torch.uint8 or s.dim() != 2:
-        raise ValueError("%s: values are a float8_e4m3fn matrix and scales a uint8 matrix, got %s %s and %s %s" % (what, v.dtype, tuple(v.shape), s.dtype, tuple(s.shape)))
-    if b.block_rows not in (1, BLOCK) or (block_rows is not None and b.block_rows != block_rows):
-        raise ValueError("%s: blocks of %s rows are wanted, got %r" % (what, "1 or 128" if block_rows is None else block_rows, b.block_rows))
-    rows, cols = v.shape
-    if b.cols < 1 or cols < _up(b.cols, BLOCK):
-        raise ValueError("%s: %d columns of values do not hold %d columns rounded up to 128" % (what, cols, b.cols))
-    if s.shape[0] < -(-rows // b.block_rows) or s.shape[1] < _up(-(-b.cols // BLOCK), 4):
-        raise ValueError("%s: scales %s do not cover the blocks of %d x %d values" % (what, tuple(s.shape), rows, b.cols))
-    if v.stride(1) != 1 or s.stride(1) != 1:
-        raise ValueError("%s: columns have to be contiguous (stride 1)" % what)
+    if v.dtype is not E4M3 or v.dim() != 2 or s.dtype is not _UINT8 or s.dim() != 2:
+        return ValueError("%s: values are a float8_e4m3fn matrix and scales a uint8 matrix, got %s %s and %s %s" % (what, v.dtype, tuple(v.shape), s.dtype, tuple(s.shape)))
+    if b.block_rows not in block_rows:
+        return ValueError("%s: blocks of %s rows are wanted, got %r" % (what, " or ".join(map(str, block_rows)), b.block_rows))
+    if b.cols < 1 or v.shape[1] < -(-b.cols // BLOCK) * BLOCK:
+        return ValueError("%s: %d columns of values do not hold %d columns rounded up to 128" % (what, v.shape[1], b.cols))
+    if s.shape[0] < -(-v.shape[0] // b.block_rows) or s.shape[1] < -(-b.cols // 512) * 4:
+        return ValueError("%s: scales %s do not cover the blocks of %d x %d values" % (what, tuple(s.shape), v.shape[0], b.cols))
     if not v.is_cuda or v.device != s.device:
-        raise ValueError("%s: values and scales have to be in one GPU's memory, got %s and %s" % (what, v.device, s.device))
+        return ValueError("%s: values and scales have to be in one GPU's memory, got %s and %s" % (what, v.device, s.device))
+    return ValueError("%s: columns have to be contiguous (stride 1)" % what)
 
 
-def _call(device, status_of):
-    """Runs `status_of` with the device current (a torch stream number of 0 is the CURRENT device's default stream) and raises what it reports."""
-    if device.index == torch.cuda.current_device():
-        status = status_of()
+def _blocks(b, what, block_rows):
+    """(rows, cols, row stride of the values, of the scales, device index); block_rows: the ones that may be"""
+    v, s, cols, br = b.values, b.scale, b.cols, b.block_rows
+    vs, ss = v.shape, s.shape
+    if (v.dtype is not E4M3 or s.dtype is not _UINT8 or len(vs) != 2 or len(ss) != 2 or br not in block_rows or cols < 1 or vs[1] < -(-cols // BLOCK) * BLOCK or
+            ss[0] * br < vs[0] or ss[1] < -(-cols // 512) * 4 or not v.is_cuda or v.get_device() != s.get_device() or v.stride(1) != 1 or s.stride(1) != 1):
+        raise _bad_blocks(b, what, block_rows)
+    return vs[0], cols, v.stride(0), s.stride(0), v.get_device()
+
+
+def _call(index, fn, *args):
+    """The entry with the tensors' device current: a torch stream number of 0 is the CURRENT device's default stream."""
+    if _devices == 1 or index == torch.cuda.current_device():
+        status = fn(*args)
     else:
-        with torch.cuda.device(device):
-            status = status_of()
+        with torch.cuda.device(index):
+            status = fn(*args)
     if status != 0:
         raise RuntimeError("block operator failed with '%s' (0x%X)" % (native.error_message(status), status))
 
 
-def _empty(rows, cols, block_rows, device):
-    values = torch.empty((rows, _up(cols, BLOCK)), dtype=E4M3, device=device)
-    scale = torch.empty((-(-rows // block_rows), _up(-(-cols // BLOCK), 4)), dtype=torch.uint8, device=device)
-    return BlockTensor(values, scale, cols, block_rows)
-
-
 def quantize_blocks(x, block_rows=1):
     """x [rows][cols] float32 / float16 / bfloat16 -> BlockTensor in blocks of block_rows (1: activations, 128: weights) x 128."""
-    _plain(x, "x")
-    if block_rows not in (1, BLOCK):
+    kind, rows, cols, ld, index = _plain(x, "x")
+    if block_rows != 1 and block_rows != BLOCK:
         raise ValueError("blocks have 1 or 128 rows, got %r" % (block_rows,))
-    rows, cols = x.shape
-    if cols < 1:
-        raise ValueError("x: at least one column is wanted")
-    b = _empty(rows, cols, block_rows, x.device)
-    L = native.lib()
-    _call(x.device, lambda: L.STTX_QuantizeBlocks(x.data_ptr(), _TYPES[x.dtype], rows, cols, x.stride(0), block_rows, b.values.data_ptr(), b.values.stride(0),
-                                                  b.scale.data_ptr(), b.scale.stride(0), torch.cuda.current_stream(x.device).cuda_stream))
-    return b
+    ldq, lds = -(-cols // BLOCK) * BLOCK, -(-cols // 512) * 4
+    values = x.new_empty((rows, ldq), dtype=E4M3)
+    scale = x.new_empty((-(-rows // block_rows), lds), dtype=_UINT8)
+    _call(index, (_lib or _entry()).STTX_QuantizeBlocks, x.data_ptr(), kind, rows, cols, ld, block_rows, values.data_ptr(), ldq, scale.data_ptr(), lds, _raw_stream(index))
+    return BlockTensor(values, scale, cols, block_rows)
 
 
 def dequantize_blocks(b, dtype=torch.float32):
     """BlockTensor -> [rows][cols] of `dtype` (float32, float16, bfloat16), one rounding."""
-    _blocks(b, "b")
-    if dtype not in _TYPES or dtype is E4M3:
+    rows, cols, ldq, lds, index = _blocks(b, "b", (1, BLOCK))
+    kind = _PLAIN.get(dtype, -1)
+    if kind < 0:
         raise ValueError("dtype: float32, float16 or bfloat16 is wanted, got %s" % (dtype,))
-    rows, cols = b.shape
-    y = torch.empty((rows, cols), dtype=dtype, device=b.values.device)
-    L = native.lib()
-    _call(y.device, lambda: L.STTX_DequantizeBlocks(b.values.data_ptr(), b.values.stride(0), b.scale.data_ptr(), b.scale.stride(0), rows, cols, b.block_rows, y.data_ptr(),
-                                                    _TYPES[dtype], y.stride(0), torch.cuda.current_stream(y.device).cuda_stream))
+    y = b.scale.new_empty((rows, cols), dtype=dtype)
+    _call(index, (_lib or _entry()).STTX_DequantizeBlocks, b.values.data_ptr(), ldq, b.scale.data_ptr(), lds, rows, cols, b.block_rows, y.data_ptr(), kind, cols, _raw_stream(index))
     return y
 
 
@@ -116,50 +133,41 @@ def dense_blocks(x, w, bias=None, relu_clip=None, dtype=torch.float16):
 
     x: [rows][in] float32 / float16 / bfloat16 (quantised within the call) or a BlockTensor in blocks of 1 x 128; w: BlockTensor [out][in] in blocks of
     128 x 128; bias: float32 [out].  Returns [rows][out] of `dtype`, or for dtype float8_e4m3fn a BlockTensor in blocks of 1 x 128."""
-    _blocks(w, "w", BLOCK)
-    out, inner = w.shape
-    if out < 1:
-        raise ValueError("w: at least one row is wanted")
-    device = w.values.device
-    a = native.DenseBlocksArgs()
+    out, inner, w_ld, w_scale_ld, index = _blocks(w, "w", (BLOCK,))
     if isinstance(x, BlockTensor):
-        _blocks(x, "x", 1)
-        a.x, a.x_scale, a.x_type = x.values.data_ptr(), x.scale.data_ptr(), 3
-        a.x_ld, a.x_scale_ld = x.values.stride(0), x.scale.stride(0)
-        at = x.values.device
+        rows, cols, x_ld, x_scale_ld, at = _blocks(x, "x", (1,))
+        kind, x_ptr, x_scale = _E4M3, x.values.data_ptr(), x.scale.data_ptr()
     else:
-        _plain(x, "x")
-        a.x, a.x_type, a.x_ld = x.data_ptr(), _TYPES[x.dtype], x.stride(0)
-        at = x.device
-    rows = x.shape[0]
-    if x.shape[1] != inner:
-        raise ValueError("x has %d columns, w has %d" % (x.shape[1], inner))
-    if at != device:
-        raise ValueError("x is on %s, w on %s" % (at, device))
+        kind, rows, cols, x_ld, at = _plain(x, "x")
+        x_ptr, x_scale, x_scale_ld = x.data_ptr(), 0, 0
+    if cols != inner or out < 1:
+        raise ValueError("x has %d columns, w is %d x %d" % (cols, out, inner))
+    if at != index:
+        raise ValueError("x is on device %d, w on device %d" % (at, index))
+    b_ptr = 0
     if bias is not None:
-        if bias.dtype is not torch.float32 or bias.dim() != 1 or bias.shape[0] != out or (bias.stride(0) != 1 and out > 1) or bias.device != device:
-            raise ValueError("bias: a contiguous float32 vector of %d on %s is wanted, got %s %s on %s" % (out, device, bias.dtype, tuple(bias.shape), bias.device))
-        a.bias = bias.data_ptr()
+        if bias.dtype is not torch.float32 or bias.dim() != 1 or bias.shape[0] != out or bias.get_device() != index or (bias.stride(0) != 1 and out > 1):
+            raise ValueError("bias: a contiguous float32 vector of %d on device %d is wanted, got %s %s on %s" % (out, index, bias.dtype, tuple(bias.shape), bias.device))
+        b_ptr = bias.data_ptr()
+    clip = 0.0
     if relu_clip is not None:
         if not relu_clip > 0.0:
             raise ValueError("relu_clip: a positive number or None is wanted, got %r" % (relu_clip,))
-        a.relu_clip = relu_clip
-    if dtype not in _TYPES:
-        raise ValueError("dtype: float32, float16, bfloat16 or float8_e4m3fn is wanted, got %s" % (dtype,))
+        clip = relu_clip
+    L = _lib or _entry()
+    need = L.STTX_DenseBlocksWorkspace(kind, rows, inner) if kind != _E4M3 else 0
+    work = w.scale.new_empty(need) if need else None         # torch's allocator: this stream's, or the capturing graph's own
     if dtype is E4M3:
-        y = _empty(rows, out, 1, device)
-        a.y, a.y_ld, a.y_scale, a.y_scale_ld = y.values.data_ptr(), y.values.stride(0), y.scale.data_ptr(), y.scale.stride(0)
+        y_ld, y_scale_ld = -(-out // BLOCK) * BLOCK, -(-out // 512) * 4
+        y = BlockTensor(w.scale.new_empty((rows, y_ld), dtype=E4M3), w.scale.new_empty((rows, y_scale_ld), dtype=_UINT8), out)
+        y_kind, y_ptr, y_scale = _E4M3, y.values.data_ptr(), y.scale.data_ptr()
     else:
-        y = torch.empty((rows, out), dtype=dtype, device=device)
-        a.y, a.y_ld = y.data_ptr(), out
-    a.y_type = _TYPES[dtype]
-    a.w, a.w_ld, a.w_scale, a.w_scale_ld = w.values.data_ptr(), w.values.stride(0), w.scale.data_ptr(), w.scale.stride(0)
-    a.rows, a.inner, a.out = rows, inner, out
-    L = native.lib()
-    need = L.STTX_DenseBlocksWorkspace(a.x_type, rows, inner)
-    if need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)     # torch's allocator: this stream's, or the capturing graph's own
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
-    a.stream = torch.cuda.current_stream(device).cuda_stream
-    _call(device, lambda: L.STTX_DenseBlocks(C.byref(a)))
+        y_kind = _PLAIN.get(dtype, -1)
+        if y_kind < 0:
+            raise ValueError("dtype: float32, float16, bfloat16 or float8_e4m3fn is wanted, got %s" % (dtype,))
+        y = w.scale.new_empty((rows, out), dtype=dtype)
+        y_ptr, y_ld, y_scale, y_scale_ld = y.data_ptr(), out, 0, 0
+    args = native.DenseBlocksArgs(x_ptr, x_scale, w.values.data_ptr(), w.scale.data_ptr(), b_ptr, y_ptr, y_scale, work.data_ptr() if need else 0, _raw_stream(index),
+                                  x_ld, x_scale_ld, w_ld, w_scale_ld, y_ld, y_scale_ld, need, rows, inner, out, kind, y_kind, clip)
+    _call(index, L.STTX_DenseBlocks, C.byref(args))
     return y
