@@ -208,8 +208,8 @@ typedef struct STTX_DenseBlocksArgs {
   float relu_clip;                  /* 0: no ReLU */
 } STTX_DenseBlocksArgs;
 STTX_EXPORT int STTX_DenseBlocks(const STTX_DenseBlocksArgs* aArgs);
-/* Bytes of workspace such a call needs (0 for x in blocks, and for few rows: those are quantised on the way into the product). */
-STTX_EXPORT unsigned long long STTX_DenseBlocksWorkspace(int aXType, long long aRows, long long aIn);
+/* Bytes of workspace such a call needs (0 for x in blocks and y not, and for others depending on the sizes). */
+STTX_EXPORT unsigned long long STTX_DenseBlocksWorkspace(int aXType, int aYType, long long aRows, long long aIn, long long aOut);
 
 /* ---- decoder on caller-supplied emissions ----------------------------------------------------- */
 typedef struct STTX_Decoder STTX_Decoder;

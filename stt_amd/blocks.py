@@ -155,8 +155,6 @@ def dense_blocks(x, w, bias=None, relu_clip=None, dtype=torch.float16):
             raise ValueError("relu_clip: a positive number or None is wanted, got %r" % (relu_clip,))
         clip = relu_clip
     L = _lib or _entry()
-    need = L.STTX_DenseBlocksWorkspace(kind, rows, inner) if kind != _E4M3 else 0
-    work = w.scale.new_empty(need) if need else None         # torch's allocator: this stream's, or the capturing graph's own
     if dtype is E4M3:
         y_ld, y_scale_ld = -(-out // BLOCK) * BLOCK, -(-out // 512) * 4
         y = BlockTensor(w.scale.new_empty((rows, y_ld), dtype=E4M3), w.scale.new_empty((rows, y_scale_ld), dtype=_UINT8), out)
@@ -167,6 +165,8 @@ def dense_blocks(x, w, bias=None, relu_clip=None, dtype=torch.float16):
             raise ValueError("dtype: float32, float16, bfloat16 or float8_e4m3fn is wanted, got %s" % (dtype,))
         y = w.scale.new_empty((rows, out), dtype=dtype)
         y_ptr, y_ld, y_scale, y_scale_ld = y.data_ptr(), out, 0, 0
+    need = L.STTX_DenseBlocksWorkspace(kind, y_kind, rows, inner, out) if kind != _E4M3 or y_kind == _E4M3 else 0
+    work = w.scale.new_empty(need) if need else None         # torch's allocator: this stream's, or the capturing graph's own
     args = native.DenseBlocksArgs(x_ptr, x_scale, w.values.data_ptr(), w.scale.data_ptr(), b_ptr, y_ptr, y_scale, work.data_ptr() if need else 0, _raw_stream(index),
                                   x_ld, x_scale_ld, w_ld, w_scale_ld, y_ld, y_scale_ld, need, rows, inner, out, kind, y_kind, clip)
     _call(index, L.STTX_DenseBlocks, C.byref(args))

@@ -108,9 +108,10 @@ int STTX_DequantizeBlocks(const unsigned char* aQ, long long aLdQ, const unsigne
   });
 }
 
-unsigned long long STTX_DenseBlocksWorkspace(int aXType, long long aRows, long long aIn) {
-  if (!plain(aXType) || aRows < 1 || aRows > kMaxRows || aIn < 1 || aIn > kMaxCols || blocks_dense_fused(aRows)) return 0;
-  return (unsigned long long)(aRows * (up(aIn, 128) + up(up(aIn, 128) / 128, 4)));
+unsigned long long STTX_DenseBlocksWorkspace(int aXType, int aYType, long long aRows, long long aIn, long long aOut) {
+  const auto type = [](int t) { return plain(t) || t == STTX_E4M3; };
+  if (!type(aXType) || !type(aYType) || aRows < 1 || aRows > kMaxRows || aIn < 1 || aIn > kMaxCols || aOut < 1 || aOut > kMaxCols) return 0;
+  return blocks_dense_workspace(aXType, aYType, aRows, (int)aOut, (int)aIn);
 }
 
 int STTX_DenseBlocks(const STTX_DenseBlocksArgs* aArgs) {
@@ -127,7 +128,7 @@ int STTX_DenseBlocks(const STTX_DenseBlocksArgs* aArgs) {
     else want_plain(c.y, c.y_type, c.rows, c.out, c.y_ld, true);
     want(c.relu_clip > 0.0f || c.relu_clip == 0.0f, "the clip of the ReLU is positive, or 0 for no ReLU");
     if (c.rows == 0) return;
-    const unsigned long long need = STTX_DenseBlocksWorkspace(c.x_type, c.rows, c.in);
+    const unsigned long long need = STTX_DenseBlocksWorkspace(c.x_type, c.y_type, c.rows, c.in, c.out);
     want(need == 0 || (c.workspace != nullptr && aligned(c.workspace, 16) && c.workspace_bytes >= need), "workspace too small (STTX_DenseBlocksWorkspace) or not aligned to 16 bytes");
     const hipStream_t st = static_cast<hipStream_t>(c.stream);
     OnDeviceOf on(st);
@@ -137,16 +138,7 @@ int STTX_DenseBlocks(const STTX_DenseBlocksArgs* aArgs) {
     a.N = (int)c.out; a.K = (int)c.in; a.x_type = c.x_type; a.y_type = c.y_type; a.relu = c.relu_clip > 0.0f; a.clip = c.relu_clip;
     if (c.x_type != STTX_E4M3) a.xvec = vec16(c.x, c.x_type, c.x_ld);
     if (c.y_type != STTX_E4M3) a.vec = aligned(c.y, 4 * elem(c.y_type)) && c.y_ld % 4 == 0;
-    if (need) {
-      BlocksQuantArgs q{};
-      q.x = c.x; q.rows = c.rows; q.ldx = c.x_ld; q.ldq = up(c.in, 128); q.lds = up(q.ldq / 128, 4);
-      q.q = static_cast<unsigned char*>(c.workspace); q.scale = q.q + c.rows * q.ldq;
-      q.cols = (int)c.in; q.type = c.x_type; q.block_rows = 1; q.vec = a.xvec;
-      launch_blocks_quantize(q, st);
-      HIP_CHECK(hipGetLastError());
-      a.x = q.q; a.x_scale = q.scale; a.ldx = q.ldq; a.ldxs = q.lds; a.x_type = BLOCKS_E4M3;
-    }
-    launch_blocks_dense(a, st);
+    launch_blocks_dense(a, c.workspace, st);
     HIP_CHECK(hipGetLastError());
   });
 }

@@ -153,7 +153,7 @@ struct BlocksDequantArgs {
   int vec;                  // rows of y may be written 16 bytes at a time
 };
 struct BlocksDenseArgs {
-  const void* x;            // [M][ldx]: e4m3 in blocks of 1 x 128 with x_scale, or f32 / f16 / bf16 (blocks_dense_fused(M) only)
+  const void* x;            // [M][ldx]: e4m3 in blocks of 1 x 128 with x_scale, or f32 / f16 / bf16, quantised so by the launch
   const unsigned char *x_scale, *w, *w_scale;   // w [N][ldw] in blocks of 128 x 128
   const float* bias;        // [N] or null
   void* y;                  // [M][ldy] f32 / f16 / bf16, or e4m3 in blocks of 1 x 128 with y_scale
@@ -166,8 +166,8 @@ struct BlocksDenseArgs {
 };
 void launch_blocks_quantize(const BlocksQuantArgs& a, hipStream_t st);
 void launch_blocks_dequantize(const BlocksDequantArgs& a, hipStream_t st);
-bool blocks_dense_fused(int64_t M);   // launch_blocks_dense quantises this many rows itself; more have to be in blocks already
-void launch_blocks_dense(const BlocksDenseArgs& a, hipStream_t st);
+size_t blocks_dense_workspace(int x_type, int y_type, int64_t M, int N, int K);   // bytes, at a multiple of 16
+void launch_blocks_dense(const BlocksDenseArgs& a, void* workspace, hipStream_t st);
 
 // dst/src: device-addressable (HBM or mapped page-locked host memory); any size, any alignment
 void launch_copy_bytes(void* dst, const void* src, size_t bytes, hipStream_t st);

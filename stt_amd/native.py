@@ -182,7 +182,7 @@ def lib():
         "STTX_QuantizeBlocks": (ci, [vp, ci, cl, cl, cl, ci, vp, cl, vp, cl, vp]),
         "STTX_DequantizeBlocks": (ci, [vp, cl, vp, cl, cl, cl, ci, vp, ci, cl, vp]),
         "STTX_DenseBlocks": (ci, [pp(DenseBlocksArgs)]),
-        "STTX_DenseBlocksWorkspace": (C.c_ulonglong, [ci, cl, cl]),
+        "STTX_DenseBlocksWorkspace": (C.c_ulonglong, [ci, ci, cl, cl, cl]),
         "STTX_TestFleetRecords": (pp(vp), [pp(cs), pp(cu), cu, cu]),
         "STTX_DebugFleetFailShard": (ci, [vp, ci]),
     }

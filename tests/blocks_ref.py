@@ -36,13 +36,9 @@ def quantize(x, block_rows):
     finite = np.isfinite(t)
     top = np.where(finite, np.abs(t), 0.0).max((1, 3))
     byte = np.full((R // block_rows, up(K // BLOCK, 4)), 127, np.int64)
-    for i in range(top.shape[0]):
-        for j in range(top.shape[1]):
-            if top[i, j] > 0:
-                e = -127
-                while top[i, j] > np.ldexp(448.0, e):
-                    e += 1
-                byte[i, j] = e + 127
+    m, e = np.frexp(top)                                     # top = m 2^e, 1/2 <= m < 1; 448 = 0.875 * 2^9: the smallest power p >= -127 with top <= 448 * 2^p
+    power = np.maximum(e - 9 + (m > 0.875), -127)
+    byte[:, :K // BLOCK] = np.where(top > 0, power + 127, 127)
     s = byte[:, None, :K // BLOCK, None] - 127
     v = np.where(finite, round_e4m3(np.ldexp(np.where(finite, t, 0.0), -s)), np.nan)
     return v.reshape(R, K)[:rows], byte.astype(np.uint8)

@@ -28,6 +28,12 @@ def test_reference_powers():
         x = np.zeros((1, 130))
         x[0, 5] = -np.float64(np.float32(top))
         assert R.quantize(x, 1)[1][0].tolist() == [byte, 127, 127, 127], top
+    rng = np.random.RandomState(1)
+    for top in np.float64(np.float32(np.concatenate([np.ldexp(rng.uniform(0.5, 1, 200), rng.randint(-148, 129, 200)), np.ldexp(448.0, rng.randint(-127, 119, 40))]))):
+        p = -127
+        while top > np.ldexp(448.0, p):
+            p += 1
+        assert R.quantize(np.full((1, 1), top), 1)[1][0, 0] == p + 127, top
 
 
 def _quant(L, x=0x10000, type=0, rows=4, cols=200, ldx=200, block_rows=1, q=0x20000, ldq=256, scale=0x30000, lds=4):
@@ -72,8 +78,9 @@ def test_dense_refuses(L, capfd):
                 dict(x_scale_ld=2), dict(w=None), dict(w_scale=None), dict(w=0x30004), dict(w_ld=250), dict(w_scale_ld=1), dict(bias=0x50002), dict(y=None), dict(y=0x60002), dict(y_ld=299),
                 dict(y_type=5), dict(y_type=3, y_ld=384), dict(y_type=3, y_ld=300, y_scale=0x70000, y_scale_ld=4), dict(y_type=3, y_ld=384, y_scale=0x70000, y_scale_ld=3),
                 dict(relu_clip=-1.0), dict(relu_clip=float("nan")),
-                dict(x_type=1, x_ld=200),                                                  # 70 rows of f16 need a workspace
-                dict(x_type=1, x_ld=200, workspace=0x80000, workspace_bytes=70 * 260 - 1), dict(x_type=1, x_ld=200, workspace=0x80004, workspace_bytes=1 << 20)):
+                dict(x_type=1, x_ld=200, rows=7000),                                       # 7000 rows of f16 need a workspace
+                dict(x_type=1, x_ld=200, rows=7000, workspace=0x80000, workspace_bytes=7000 * 260 - 1), dict(x_type=1, x_ld=200, rows=7000, workspace=0x80004, workspace_bytes=1 << 30),
+                dict(y_type=3, y_ld=384, y_scale=0x70000, y_scale_ld=4, workspace=0x80000, workspace_bytes=70 * 300 * 4 - 1)):
         assert _dense(L, **bad) == INVALID_SHAPE, bad
         assert "STTX_DenseBlocks" in capfd.readouterr().err, bad
     assert L.STTX_DenseBlocks(None) == INVALID_SHAPE
@@ -81,11 +88,13 @@ def test_dense_refuses(L, capfd):
 
 
 def test_workspace(L):
-    assert L.STTX_DenseBlocksWorkspace(3, 1 << 20, 2048) == 0            # already in blocks
-    assert L.STTX_DenseBlocksWorkspace(0, 1, 2048) == 0                  # few rows are quantised on the way
-    assert L.STTX_DenseBlocksWorkspace(1, 6144, 494) == 6144 * (512 + 4)
-    assert L.STTX_DenseBlocksWorkspace(2, 1 << 20, 130) == (1 << 20) * (256 + 4)
-    assert L.STTX_DenseBlocksWorkspace(9, 100, 100) == 0 and L.STTX_DenseBlocksWorkspace(0, -1, 100) == 0
+    W = L.STTX_DenseBlocksWorkspace
+    assert W(3, 0, 1 << 20, 2048, 8192) == 0                  # already in blocks
+    assert W(0, 1, 1, 2048, 2048) == 0                        # few rows are quantised on the way
+    assert W(3, 3, 16, 2048, 2046) == 16 * 2048 * 4           # ... and their results, where those go on in blocks
+    assert W(1, 0, 6144, 494, 2048) == 6144 * (512 + 4) == W(1, 3, 6144, 494, 2048)
+    assert W(2, 2, 1 << 20, 130, 2048) == (1 << 20) * (256 + 4)
+    assert W(9, 0, 100, 100, 100) == 0 and W(0, 0, -1, 100, 100) == 0 and W(0, -1, 5000, 100, 9000) == 0 and W(0, 0, 5000, 0, 9000) == 0
 
 
 def test_python_refuses():
