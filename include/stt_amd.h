@@ -264,7 +264,8 @@ STTX_EXPORT int STTX_ReadModelTensor(const char* aModelBuffer, unsigned int aBuf
 /* (the kernel-level test hooks -- STTX_Test*, STTX_Debug* -- are declared in include/stt_amd_test.h and exist in libstt_test.so only) */
 /* Which arithmetic the acoustic model of aCtx runs in: 0 = f16 MFMA operands / f32 accumulate (north_star's; int8 weights of a quantised
  * file are de-quantised), 1 = the released models' own (TensorFlow Lite's hybrid int8 FULLY_CONNECTED end to end: int8 activations per row,
- * int32 sums; taken for a dynamic-range quantised `.tflite`, or with the tunable am_i8 = 1).  Replaces nothing in coqui-stt.h: the
+ * int32 sums; taken for a dynamic-range quantised `.tflite`, or with the tunable am_i8 = 1), 2 = layers 1-3, the x half of the cell and layer 5 as
+ * STTX_DenseBlocks runs them, everything else as in 0 (taken with the tunable am_f8 = 1 when the model is loaded, for any file).  Replaces nothing in coqui-stt.h: the
  * reference's CPU path has only the second one (native_client/tflitemodelstate.cc:200,369-405). */
 STTX_EXPORT int STTX_GetAcousticMode(const ModelState* aCtx);
 /* Host-side packing of the recurrent matrix (no GPU needed): aKernel [2H][4H] f32 -> aOut [4H*H] f16 bits. */

@@ -1451,7 +1451,7 @@ int STTX_TestDense(int M, int N, int K, const float* aX, const float* aW, const 
 // TFLite's hybrid FULLY_CONNECTED on the int8 MFMA path (kernels.h: launch_quantize_rows + launch_dense_hybrid_i8), as a test hook:
 // x f32 [M][K], wq int8 [N][K], wscale [n_scales = 1 or N], bias [N] -> y f32 [M][N] (and, if asked for, the quantised rows and their
 // scales); aReps timed repetitions of quantisation + product (HIP events) -> *aElapsedMs per repetition.
-int STTX_GetAcousticMode(const ModelState* m) { return m && m->i8 ? 1 : 0; }
+int STTX_GetAcousticMode(const ModelState* m) { return m ? m->arithmetic() : 0; }
 #ifdef STT_TEST_HOOKS
 int STTX_DebugSlowRows(ModelState* m, unsigned int* aRows) {
   return guarded([&]() {
@@ -1579,6 +1579,7 @@ int STTX_TestLstmSteps(ModelState* m, unsigned int aBatch, unsigned int aSteps, 
     const int n_co = tune().lstm_cotenant;
     auto cotenant = [&]() {
       if (n_co <= 0) return;
+      if (m->f8) throw std::runtime_error("lstm_cotenant: the model's x-projection is not held in f16 (am_f8)");
       const int M = 6144;
       cx.reserve((size_t)M * H * 2); cy.reserve((size_t)M * 4 * H * 4);
       HIP_CHECK(hipMemsetAsync(cx.p, 0, (size_t)M * H * 2, m->stream));

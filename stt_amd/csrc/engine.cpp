@@ -110,6 +110,36 @@ static void acoustic_rows_i8(ModelState& m, const float* d_x1, int B, int T, flo
   launch_softmax(s, st);
 }
 
+// Rows in blocks of 1 x 128 in one buffer: values [M][N rounded up to 128], then their scale bytes.
+static int64_t blocks_ld(int N) { return (N + 127) / 128 * 128; }
+static int64_t blocks_lds(int N) { return (N + 511) / 512 * 4; }
+static size_t blocks_bytes(int M, int N) { return (size_t)M * (blocks_ld(N) + blocks_lds(N)); }
+// One dense layer in blocks: x f16 [M][ldx] or rows in blocks (ldx 0), y f32 / f16 [M][N] or rows in blocks.
+static void f8_dense(const ModelState::BlocksMatrix& w, const float* bias, const void* x, int x_type, int ldx, int M, void* y, int y_type, float clip, DevBuf& work,
+                     int lds_floor, hipStream_t st) {
+  BlocksDenseArgs a{};
+  a.M = M; a.N = w.N; a.K = w.K; a.x = x; a.x_type = x_type; a.ldx = ldx;
+  if (x_type == BLOCKS_E4M3) { a.ldx = blocks_ld(w.K); a.ldxs = blocks_lds(w.K); a.x_scale = static_cast<const unsigned char*>(x) + M * a.ldx; }
+  else a.xvec = ldx % 8 == 0;
+  a.w = w.values.as<unsigned char>(); a.w_scale = w.scale.as<unsigned char>(); a.ldw = blocks_ld(w.K); a.ldws = blocks_lds(w.K);
+  a.bias = bias; a.y = y; a.y_type = y_type; a.ldy = w.N; a.vec = w.N % 4 == 0;
+  if (y_type == BLOCKS_E4M3) { a.ldy = blocks_ld(w.N); a.ldys = blocks_lds(w.N); a.y_scale = static_cast<unsigned char*>(y) + M * a.ldy; }
+  a.relu = clip > 0.0f; a.clip = clip; a.lds_floor = lds_floor;
+  a.ordered = 1;      // transcripts do not depend on how utterances and streams were grouped
+  work.reserve(blocks_dense_workspace(x_type, y_type, M, w.N, w.K, 1));
+  launch_blocks_dense(a, work.p, st);
+}
+void ModelState::f8_front(const _Float16* x1, int ldx, int M, DevBuf& a, DevBuf& b, DevBuf& work, float* xproj, int lds_floor, hipStream_t st) {
+  a.reserve(blocks_bytes(M, g.n_hidden)); b.reserve(blocks_bytes(M, g.n_hidden));
+  f8_dense(f1, b1.as<float>(), x1, BLOCKS_F16, ldx, M, a.p, BLOCKS_E4M3, g.relu_clip, work, lds_floor, st);
+  f8_dense(f2, b2.as<float>(), a.p, BLOCKS_E4M3, 0, M, b.p, BLOCKS_E4M3, g.relu_clip, work, lds_floor, st);
+  f8_dense(f3, b3.as<float>(), b.p, BLOCKS_E4M3, 0, M, a.p, BLOCKS_E4M3, g.relu_clip, work, lds_floor, st);
+  f8_dense(fx, bl.as<float>(), a.p, BLOCKS_E4M3, 0, M, xproj, BLOCKS_F32, 0.0f, work, lds_floor, st);
+}
+void ModelState::f8_layer5(const _Float16* h, int M, DevBuf& work, _Float16* y, int lds_floor, hipStream_t st) {
+  f8_dense(f5, b5.as<float>(), h, BLOCKS_F16, g.n_hidden, M, y, BLOCKS_F16, g.relu_clip, work, lds_floor, st);
+}
+
 static void acoustic_rows(ModelState& m, const void* d_x1v, int B, int T, float* d_c, float* d_h, int carry, int t_par,
                           float* d_probs_out, int probs_t_max, const int* d_nframes = nullptr) {
   if (m.i8) { acoustic_rows_i8(m, static_cast<const float*>(d_x1v), B, T, d_c, d_h, carry, d_probs_out, probs_t_max, d_nframes, t_par); return; }
@@ -129,15 +159,18 @@ static void acoustic_rows(ModelState& m, const void* d_x1v, int B, int T, float*
   d.relu_clip = g.relu_clip; d.M = M;
   stt_prof_mark(&m, 1);
   // layers 1-3 (deepspeech_model.py:204-224)
-  d.wt = m.w1t.as<_Float16>(); d.x = d_x1; d.bias = m.b1.as<float>(); d.y = m.ws_a.p; d.N = H; d.K = g.k1_pad(); d.ldx = g.k1_pad(); d.ldy = H;
-  launch_dense(d, DENSE_EPI_RELU_F16, stream);
-  d.wt = m.w2t.as<_Float16>(); d.x = m.ws_a.as<_Float16>(); d.bias = m.b2.as<float>(); d.y = m.ws_b.p; d.K = H; d.ldx = H;
-  launch_dense(d, DENSE_EPI_RELU_F16, stream);
-  d.wt = m.w3t.as<_Float16>(); d.x = m.ws_b.as<_Float16>(); d.bias = m.b3.as<float>(); d.y = m.ws_a.p;
-  launch_dense(d, DENSE_EPI_RELU_F16, stream);
-  // x-projection of all timesteps at once: [M][H] x [H][4H] + lstm bias
-  d.wt = m.wxt.as<_Float16>(); d.x = m.ws_a.as<_Float16>(); d.bias = m.bl.as<float>(); d.y = m.ws_xproj.p; d.N = 4 * H; d.ldy = 4 * H;
-  launch_dense(d, DENSE_EPI_BIAS_F32, stream);
+  if (m.f8) m.f8_front(d_x1, g.k1_pad(), M, m.f8_a, m.f8_b, m.f8_work, m.ws_xproj.as<float>(), 0, stream);
+  else {
+    d.wt = m.w1t.as<_Float16>(); d.x = d_x1; d.bias = m.b1.as<float>(); d.y = m.ws_a.p; d.N = H; d.K = g.k1_pad(); d.ldx = g.k1_pad(); d.ldy = H;
+    launch_dense(d, DENSE_EPI_RELU_F16, stream);
+    d.wt = m.w2t.as<_Float16>(); d.x = m.ws_a.as<_Float16>(); d.bias = m.b2.as<float>(); d.y = m.ws_b.p; d.K = H; d.ldx = H;
+    launch_dense(d, DENSE_EPI_RELU_F16, stream);
+    d.wt = m.w3t.as<_Float16>(); d.x = m.ws_b.as<_Float16>(); d.bias = m.b3.as<float>(); d.y = m.ws_a.p;
+    launch_dense(d, DENSE_EPI_RELU_F16, stream);
+    // x-projection of all timesteps at once: [M][H] x [H][4H] + lstm bias
+    d.wt = m.wxt.as<_Float16>(); d.x = m.ws_a.as<_Float16>(); d.bias = m.bl.as<float>(); d.y = m.ws_xproj.p; d.N = 4 * H; d.ldy = 4 * H;
+    launch_dense(d, DENSE_EPI_BIAS_F32, stream);
+  }
   stt_prof_mark(&m, 2);
   // recurrence
   float* cbuf = (carry != 2 && d_c) ? d_c : m.ws_c.as<float>();
@@ -158,10 +191,13 @@ static void acoustic_rows(ModelState& m, const void* d_x1v, int B, int T, float*
   }
   stt_prof_mark(&m, 3);
   // layer 5, layer 6, softmax (deepspeech_model.py:241-252, 357)
-  d.wt = m.w5t.as<_Float16>(); d.x = m.ws_hall.as<_Float16>(); d.bias = m.b5.as<float>(); d.y = m.ws_b.p; d.N = H; d.K = H; d.ldx = H; d.ldy = H;
-  launch_dense(d, DENSE_EPI_RELU_F16, stream);
+  if (m.f8) m.f8_layer5(m.ws_hall.as<_Float16>(), M, m.f8_work, m.ws_b.as<_Float16>(), 0, stream);
+  else {
+    d.wt = m.w5t.as<_Float16>(); d.x = m.ws_hall.as<_Float16>(); d.bias = m.b5.as<float>(); d.y = m.ws_b.p; d.N = H; d.K = H; d.ldx = H; d.ldy = H;
+    launch_dense(d, DENSE_EPI_RELU_F16, stream);
+  }
   if (!launch_logits_softmax(m.ws_b.as<_Float16>(), m.w6t.as<_Float16>(), m.b6.as<float>(), d_probs_out, M, H, C, B, probs_t_max, stream)) {
-    d.wt = m.w6t.as<_Float16>(); d.x = m.ws_b.as<_Float16>(); d.bias = m.b6.as<float>(); d.y = m.ws_logits.p; d.N = g.c_pad(); d.ldy = g.c_pad();
+    d.wt = m.w6t.as<_Float16>(); d.x = m.ws_b.as<_Float16>(); d.bias = m.b6.as<float>(); d.y = m.ws_logits.p; d.N = g.c_pad(); d.K = H; d.ldx = H; d.ldy = g.c_pad();
     launch_dense(d, DENSE_EPI_BIAS_F32, stream);
     SoftmaxArgs s{};
     s.logits = m.ws_logits.as<float>(); s.probs = d_probs_out; s.M = M; s.C = C; s.ldl = g.c_pad(); s.batch = B; s.t_max = probs_t_max;
@@ -595,14 +631,17 @@ void ModelState::run_acoustic_chunk_piped(const float* d_feats, const int* d_nfr
     d.solo = lstm_passes >= 2 ? solo : 0; d.lds_floor = d.solo ? 0 : dense_lds_floor();  // (96 KiB beside the one-pass step's 66 would not fit)
   }
   stt_prof_mark_on(this, 1, 0, stream);
-  d.wt = w1t.as<_Float16>(); d.x = ws_x1.as<_Float16>(); d.bias = b1.as<float>(); d.y = ws_a.p; d.N = H; d.K = g.k1_pad(); d.ldx = g.k1_pad(); d.ldy = H;
-  launch_dense(d, DENSE_EPI_RELU_F16, stream);
-  d.wt = w2t.as<_Float16>(); d.x = ws_a.as<_Float16>(); d.bias = b2.as<float>(); d.y = ws_b.p; d.K = H; d.ldx = H;
-  launch_dense(d, DENSE_EPI_RELU_F16, stream);
-  d.wt = w3t.as<_Float16>(); d.x = ws_b.as<_Float16>(); d.bias = b3.as<float>(); d.y = ws_a.p;
-  launch_dense(d, DENSE_EPI_RELU_F16, stream);
-  d.wt = wxt.as<_Float16>(); d.x = ws_a.as<_Float16>(); d.bias = bl.as<float>(); d.y = am_xproj[slot].p; d.N = 4 * H; d.ldy = 4 * H;
-  launch_dense(d, DENSE_EPI_BIAS_F32, stream);
+  if (f8) f8_front(ws_x1.as<_Float16>(), g.k1_pad(), M, am_f8a, am_f8b, am_f8work, am_xproj[slot].as<float>(), dense_lds_floor(), stream);
+  else {
+    d.wt = w1t.as<_Float16>(); d.x = ws_x1.as<_Float16>(); d.bias = b1.as<float>(); d.y = ws_a.p; d.N = H; d.K = g.k1_pad(); d.ldx = g.k1_pad(); d.ldy = H;
+    launch_dense(d, DENSE_EPI_RELU_F16, stream);
+    d.wt = w2t.as<_Float16>(); d.x = ws_a.as<_Float16>(); d.bias = b2.as<float>(); d.y = ws_b.p; d.K = H; d.ldx = H;
+    launch_dense(d, DENSE_EPI_RELU_F16, stream);
+    d.wt = w3t.as<_Float16>(); d.x = ws_b.as<_Float16>(); d.bias = b3.as<float>(); d.y = ws_a.p;
+    launch_dense(d, DENSE_EPI_RELU_F16, stream);
+    d.wt = wxt.as<_Float16>(); d.x = ws_a.as<_Float16>(); d.bias = bl.as<float>(); d.y = am_xproj[slot].p; d.N = 4 * H; d.ldy = 4 * H;
+    launch_dense(d, DENSE_EPI_BIAS_F32, stream);
+  }
   stt_prof_mark_on(this, -1, 0, stream);
   HIP_CHECK(hipEventRecord(ev_x_ready[slot], stream));
 
@@ -645,11 +684,14 @@ void ModelState::run_acoustic_chunk_piped(const float* d_feats, const int* d_nfr
   HIP_CHECK(hipStreamWaitEvent(stream_o, ev_h_ready[slot], 0));
   stt_prof_mark_on(this, 3, 6, stream_o);
   float* probs_out = d_probs + (size_t)t0 * C;
-  d.wt = w5t.as<_Float16>(); d.x = am_hall[slot].as<_Float16>(); d.bias = b5.as<float>(); d.y = ws_o.p; d.N = H; d.K = H; d.ldx = H; d.ldy = H;
-  launch_dense(d, DENSE_EPI_RELU_F16, stream_o);
+  if (f8) f8_layer5(am_hall[slot].as<_Float16>(), M, am_f8owork, ws_o.as<_Float16>(), dense_lds_floor(), stream_o);
+  else {
+    d.wt = w5t.as<_Float16>(); d.x = am_hall[slot].as<_Float16>(); d.bias = b5.as<float>(); d.y = ws_o.p; d.N = H; d.K = H; d.ldx = H; d.ldy = H;
+    launch_dense(d, DENSE_EPI_RELU_F16, stream_o);
+  }
   HIP_CHECK(hipEventRecord(ev_h_free[slot], stream_o));
   if (!launch_logits_softmax(ws_o.as<_Float16>(), w6t.as<_Float16>(), b6.as<float>(), probs_out, M, H, C, B, t_max, stream_o)) {
-    d.wt = w6t.as<_Float16>(); d.x = ws_o.as<_Float16>(); d.bias = b6.as<float>(); d.y = am_logits.p; d.N = g.c_pad(); d.ldy = g.c_pad();
+    d.wt = w6t.as<_Float16>(); d.x = ws_o.as<_Float16>(); d.bias = b6.as<float>(); d.y = am_logits.p; d.N = g.c_pad(); d.K = H; d.ldx = H; d.ldy = g.c_pad();
     launch_dense(d, DENSE_EPI_BIAS_F32, stream_o);
     SoftmaxArgs sm{};
     sm.logits = am_logits.as<float>(); sm.probs = probs_out; sm.M = M; sm.C = C; sm.ldl = g.c_pad(); sm.batch = B; sm.t_max = t_max;

@@ -228,6 +228,16 @@ struct ModelState {
   DevBuf w1q, w2q, w3q, wxq, whq, whpq, w5q, w6q;
   DevBuf s1, s2, s3, sk, s5, s6, b6q;     // b6q: the output layer's bias padded to c_pad8()
   int sn[6] = {1, 1, 1, 1, 1, 1};         // scales per matrix (1 or N)
+  // A third arithmetic, taken with the tunable am_f8 = 1: layers 1-3, the x half of the cell and layer 5 in 8-bit floating point with a power of two per
+  // block of 128 (kernels.h: BlocksDenseArgs; rows go from layer to layer in blocks, written so by the product).  The recurrent half, the cell, layer 6
+  // and the softmax are the f16 path's own.  Half the weight bytes of f16 for these five matrices.
+  bool f8 = false;
+  struct BlocksMatrix { DevBuf values, scale; int N = 0, K = 0; };
+  BlocksMatrix f1, f2, f3, fx, f5;
+  DevBuf f8_a, f8_b, f8_work, am_f8a, am_f8b, am_f8work, am_f8owork;   // rows in blocks and workspaces: one-stream paths, three engines
+  void f8_front(const _Float16* x1, int ldx, int M, DevBuf& a, DevBuf& b, DevBuf& work, float* xproj, int lds_floor, hipStream_t st);   // layers 1-3, x half of the cell
+  void f8_layer5(const _Float16* h, int M, DevBuf& work, _Float16* y, int lds_floor, hipStream_t st);
+  int arithmetic() const { return i8 ? 1 : f8 ? 2 : 0; }   // STTX_GetAcousticMode
   // workspaces of the int8 path (one-stream paths; the three-engine batch path has its own below)
   DevBuf q_x, q_s, q_rng, ws_hq0, ws_hq1, ws_hprev0, ws_pmax, ws_flag, ws_zslow, ws_hlast, ws_slow;
   // feature tables

@@ -163,10 +163,12 @@ struct BlocksDenseArgs {
   float clip;
   int xvec;                 // rows of an f32 / f16 / bf16 x may be read 16 bytes at a time
   int vec;                  // rows of y may be written four values at a time
+  int ordered;              // 1: every sum runs along k in ONE order however many rows there are (the tiled form always): a row's results do not depend on the rows beside it
+  int lds_floor;            // as DenseArgs::lds_floor
 };
 void launch_blocks_quantize(const BlocksQuantArgs& a, hipStream_t st);
 void launch_blocks_dequantize(const BlocksDequantArgs& a, hipStream_t st);
-size_t blocks_dense_workspace(int x_type, int y_type, int64_t M, int N, int K);   // bytes, at a multiple of 16
+size_t blocks_dense_workspace(int x_type, int y_type, int64_t M, int N, int K, int ordered = 0);   // bytes, at a multiple of 16
 void launch_blocks_dense(const BlocksDenseArgs& a, void* workspace, hipStream_t st);
 
 // dst/src: device-addressable (HBM or mapped page-locked host memory); any size, any alignment

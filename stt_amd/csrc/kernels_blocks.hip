@@ -593,13 +593,13 @@ int few_tiles_(int64_t M, int N) {
 
 template <int BM, int WN>
 void tile_(const BlocksDenseArgs& a, hipStream_t st) {
-  constexpr int lds = 3 * (128 + BM) * 64;
+  const int lds = max(3 * (128 + BM) * 64, min(a.lds_floor, 128 * 1024));
   const int64_t tiles = (int64_t)((a.N + 127) / 128) * ((a.M + BM - 1) / BM), grid = (tiles + 7) / 8 * 8;
   if (grid > 0x7fffffff) throw std::runtime_error("launch_blocks_dense: too many rows for one launch");
   static std::once_flag once[16];
   int dev = 0;
   (void)hipGetDevice(&dev);
-  std::call_once(once[dev & 15], []() { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(dense_tile_kernel<BM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, lds); });
+  std::call_once(once[dev & 15], []() { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(dense_tile_kernel<BM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024); });
   hipLaunchKernelGGL((dense_tile_kernel<BM, WN>), dim3((unsigned)grid), dim3(256), lds, st, a);
 }
 
@@ -643,16 +643,16 @@ void launch_blocks_dequantize(const BlocksDequantArgs& a, hipStream_t st) {
 
 // Rows that are not in blocks and go to the tiled form are quantised into the workspace first (the few-rows form quantises them on the way); y in
 // blocks from the few-rows form goes through f32 rows in the workspace, because its workgroups hold 16 of a block's 128 features.
-size_t blocks_dense_workspace(int x_type, int y_type, int64_t M, int N, int K) {
+size_t blocks_dense_workspace(int x_type, int y_type, int64_t M, int N, int K, int ordered) {
   if (M < 1) return 0;
-  if (few_tiles_(M, N)) return y_type == BLOCKS_E4M3 ? (size_t)M * (((size_t)N + 3) / 4 * 4) * 4 : 0;
+  if (!ordered && few_tiles_(M, N)) return y_type == BLOCKS_E4M3 ? (size_t)M * (((size_t)N + 3) / 4 * 4) * 4 : 0;
   return x_type == BLOCKS_E4M3 ? 0 : (size_t)M * (((size_t)K + 127) / 128 * 128 + ((size_t)K + 511) / 512 * 4);
 }
 
 void launch_blocks_dense(const BlocksDenseArgs& args, void* workspace, hipStream_t st) {
   BlocksDenseArgs a = args;
   if (a.M < 1) return;
-  if (const int mt = few_tiles_(a.M, a.N)) {
+  if (const int mt = a.ordered ? 0 : few_tiles_(a.M, a.N)) {
     if (a.y_type == BLOCKS_E4M3) { a.y = workspace; a.y_type = BLOCKS_F32; a.ldy = ((int64_t)a.N + 3) / 4 * 4; a.vec = 1; }
     switch (a.x_type) {
       case BLOCKS_F32: few_rows_<BLOCKS_F32>(a, mt, st); break;

@@ -42,6 +42,22 @@ std::vector<_Float16> transpose_f16(const float* w, int K, int N, int K_pad, int
     for (int n = 0; n < N; ++n) out[(size_t)n * K_pad + k] = (_Float16)w[(size_t)k * ldw + n];
   return out;
 }
+// W [K][N] f32 -> the same in blocks of 128 x 128, [N][K], quantised on the device
+void upload_blocks(ModelState::BlocksMatrix& m, const float* w, int K, int N, hipStream_t st) {
+  std::vector<float> t((size_t)N * K);
+  for (int k = 0; k < K; ++k)
+    for (int n = 0; n < N; ++n) t[(size_t)n * K + k] = w[(size_t)k * N + n];
+  DevBuf wide;
+  wide.upload(t.data(), t.size() * 4, st);
+  BlocksQuantArgs q{};
+  q.ldq = (K + 127) / 128 * 128; q.lds = (K + 511) / 512 * 4;
+  m.N = N; m.K = K;
+  m.values.reserve((size_t)N * q.ldq); m.scale.reserve((size_t)(N + 127) / 128 * q.lds);
+  q.x = wide.p; q.rows = N; q.cols = K; q.ldx = K; q.type = BLOCKS_F32; q.block_rows = 128; q.vec = K % 4 == 0;
+  q.q = m.values.as<unsigned char>(); q.scale = m.scale.as<unsigned char>();
+  launch_blocks_quantize(q, st);
+  HIP_CHECK(hipStreamSynchronize(st));      // (`wide` is freed here)
+}
 }  // namespace
 
 int n_frames_for(const Geometry& g, int n_samples) {  // stt.cc:105-128 + flushBuffers :236-254
@@ -193,11 +209,18 @@ int ModelState::InitFromBuffer(const char* buf, size_t len) {
   if (!stream) create_engine_stream(&stream, 0);
   if (!stream_dec) create_engine_stream(&stream_dec, 3);
   {
-    auto t = transpose_f16(l1w, K1, H, g.k1_pad(), H, H); w1t.upload(t.data(), t.size() * 2, stream);
-    t = transpose_f16(l2w, H, H, H, H, H); w2t.upload(t.data(), t.size() * 2, stream);
-    t = transpose_f16(l3w, H, H, H, H, H); w3t.upload(t.data(), t.size() * 2, stream);
-    t = transpose_f16(lk, H, 4 * H, H, 4 * H, 4 * H); wxt.upload(t.data(), t.size() * 2, stream);  // x rows of the kernel
-    t = transpose_f16(l5w, H, H, H, H, H); w5t.upload(t.data(), t.size() * 2, stream);
+    f8 = tune().am_f8 > 0;
+    std::vector<_Float16> t;
+    if (f8) {
+      upload_blocks(f1, l1w, K1, H, stream); upload_blocks(f2, l2w, H, H, stream); upload_blocks(f3, l3w, H, H, stream);
+      upload_blocks(fx, lk, H, 4 * H, stream); upload_blocks(f5, l5w, H, H, stream);
+    } else {
+      t = transpose_f16(l1w, K1, H, g.k1_pad(), H, H); w1t.upload(t.data(), t.size() * 2, stream);
+      t = transpose_f16(l2w, H, H, H, H, H); w2t.upload(t.data(), t.size() * 2, stream);
+      t = transpose_f16(l3w, H, H, H, H, H); w3t.upload(t.data(), t.size() * 2, stream);
+      t = transpose_f16(lk, H, 4 * H, H, 4 * H, 4 * H); wxt.upload(t.data(), t.size() * 2, stream);  // x rows of the kernel
+      t = transpose_f16(l5w, H, H, H, H, H); w5t.upload(t.data(), t.size() * 2, stream);
+    }
     t = transpose_f16(l6w, H, C, H, g.c_pad(), C); w6t.upload(t.data(), t.size() * 2, stream);
     std::vector<_Float16> packed((size_t)H * 4 * H);
     pack_lstm_recurrent_host(lk, H, packed.data());
@@ -211,8 +234,8 @@ int ModelState::InitFromBuffer(const char* buf, size_t len) {
   // ---- the released models' own arithmetic: the int8 matrices as the file holds them (or quantised here as the converter would)
   {
     const int want = tune().am_i8;
-    i8 = (want > 0 || (want < 0 && v.quant != nullptr)) && H % 256 == 0 && H <= 4096;
-    if ((want > 0 || (want < 0 && v.quant)) && !i8)
+    i8 = !f8 && (want > 0 || (want < 0 && v.quant != nullptr)) && H % 256 == 0 && H <= 4096;
+    if (!f8 && (want > 0 || (want < 0 && v.quant)) && !i8)
       fprintf(stderr, "Note: n_hidden = %d is outside the int8 path's shapes (multiples of 256 up to 4096): int8 weights are de-quantised to f16.\n", H);
   }
   if (i8) {
