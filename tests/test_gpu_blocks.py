@@ -199,6 +199,9 @@ def test_dense_powers_far_apart():
     y = host(blocks.dense_blocks(x, w, dtype=torch.float32))
     assert (y[1:3] == np.inf).all()
     want = R.dense(xd[[0, 3]].astype(np.float64), wd.astype(np.float64))
+    small = gpu_blocks(v, np.array([[0, 1, 127, 127]] * 4, np.uint8), 256, 1)                      # 3 * 2^-127 and 5 * 2^-126, at and above 2^-126
+    exact = 3 * 2.0 ** -127 * 3 * 2.0 ** 100 + 5 * 2.0 ** -126 * 5 * 2.0 ** -100
+    assert (np.abs(host(blocks.dense_blocks(small, w, dtype=torch.float32)) - exact) <= 2.0 ** -22 * exact).all()
     assert (np.abs(y[[0, 3]] - want) <= 2.0 ** -22 * np.abs(want)).all(), (y, want)
 
 
