@@ -95,7 +95,11 @@ template <int T> __device__ __forceinline__ void store8(const float v[8], typena
 // first taken over everything; only where that turns out not to be finite (kInf and up) is the block looked through again for its finite values.
 constexpr unsigned kInf = 0x7f800000u;
 __device__ __forceinline__ unsigned mag_(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-__device__ __forceinline__ unsigned finite_mag_(float v) { const unsigned u = mag_(v); return u < kInf ? u : 0u; }
+__device__ __forceinline__ unsigned finite_mag_(float v) {
+  asm volatile("" : "+v"(v));          // (the rare second look: without this the compiler keeps the magnitudes of the first one in as many registers)
+  const unsigned u = mag_(v);
+  return u < kInf ? u : 0u;
+}
 template <int N> __device__ __forceinline__ unsigned top_of_(const float (&v)[N], bool all) {
   unsigned t = 0;
   if (all) {
