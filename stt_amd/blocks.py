@@ -12,7 +12,7 @@ call.  No compute happens in Python; there is no fallback for tensors elsewhere.
 A call on a few rows is over in less time than a careless caller needs to make it, so the checks below are one expression each on the way that
 succeeds, and the messages are put together on the way that fails.
 """
-import ctypes as C
+import struct
 
 import torch
 
@@ -24,6 +24,7 @@ _PLAIN = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}            # ST
 _E4M3 = 3
 _UINT8 = torch.uint8
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_ARGS = struct.Struct("9Q6q1Q3q2if4x").pack                                  # native.DenseBlocksArgs as bytes: a third of the time of filling one in
 _lib = None
 
 
@@ -167,7 +168,7 @@ def dense_blocks(x, w, bias=None, relu_clip=None, dtype=torch.float16):
         y_ptr, y_ld, y_scale, y_scale_ld = y.data_ptr(), out, 0, 0
     need = L.STTX_DenseBlocksWorkspace(kind, y_kind, rows, inner, out) if kind != _E4M3 or y_kind == _E4M3 else 0
     work = w.scale.new_empty(need) if need else None         # torch's allocator: this stream's, or the capturing graph's own
-    args = native.DenseBlocksArgs(x_ptr, x_scale, w.values.data_ptr(), w.scale.data_ptr(), b_ptr, y_ptr, y_scale, work.data_ptr() if need else 0, _raw_stream(index),
+    args = _ARGS(x_ptr, x_scale, w.values.data_ptr(), w.scale.data_ptr(), b_ptr, y_ptr, y_scale, work.data_ptr() if need else 0, _raw_stream(index),
                                   x_ld, x_scale_ld, w_ld, w_scale_ld, y_ld, y_scale_ld, need, rows, inner, out, kind, y_kind, clip)
-    _call(index, L.STTX_DenseBlocks, C.byref(args))
+    _call(index, L.STTX_DenseBlocks, args)
     return y

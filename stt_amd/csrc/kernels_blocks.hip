@@ -297,13 +297,15 @@ template <> struct XQuarter<BLOCKS_E4M3> {
 };
 
 // Few rows: 16 output features by 16 MT rows per workgroup, the blocks along k dealt to its eight waves; operands straight from L2 / HBM into
-// registers, U blocks asked for at a time, the waves' sums meet in LDS (in the order of the waves: the same bits every time).  What bounds it is how
-// much one compute unit can have under way: sixteen features a workgroup put 2048 of them on 128 units (16 rows, k = 2048: 4.4 us; a block of 128
-// features a workgroup, which could write y in blocks itself, is on 16 units and takes 18.7 us).
-template <int T, int MT, int U>
+// registers, the waves' sums meet in LDS (in the order of the waves: the same bits every time).  What bounds it is how much a compute unit takes in,
+// some 30 GB/s of its part of w and of all of x: sixteen features a workgroup put 2048 of them on 128 units (16 rows, k = 2048: 4.1 us of which a
+// launch is 2; asking for two or four blocks ahead changes nothing), and a block of 128 features a workgroup, which could write y in blocks itself,
+// is on 16 units and takes 18.7 us.
+template <int T, int MT>
 __global__ __launch_bounds__(512) void dense_few_kernel(BlocksDenseArgs a) {
   constexpr int KW = 8;
   __shared__ f32x4 part[KW][MT][64];
+  __shared__ __attribute__((aligned(16))) float s_bias[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int li = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16;
@@ -312,9 +314,8 @@ __global__ __launch_bounds__(512) void dense_few_kernel(BlocksDenseArgs a) {
   const int n = min(n0 + li, a.N - 1);
   const unsigned char* wp = a.w + (int64_t)n * a.ldw + g * 32;
   const unsigned char* ws = a.w_scale + (int64_t)(n >> 7) * a.ldws;
-  int64_t m[MT];
-  __shared__ __attribute__((aligned(16))) float s_bias[16];
   if (tid < 16) s_bias[tid] = a.bias && n0 + tid < a.N ? a.bias[n0 + tid] : 0.0f;
+  int64_t m[MT];
   f32x4 acc[MT];
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
@@ -322,38 +323,28 @@ __global__ __launch_bounds__(512) void dense_few_kernel(BlocksDenseArgs a) {
     m[j] = row < a.M ? row : a.M - 1;
     acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  for (int k0 = wave; k0 < nb; k0 += KW * U) {
-    i32x4 lo[U], hi[U];
-    int wb[U];
-    XQuarter<T> x[U][MT];
+  for (int kb = wave; kb < nb; kb += KW) {
+    const i32x4* p = reinterpret_cast<const i32x4*>(wp + (int64_t)kb * 128);
+    const i32x4 lo = p[0], hi = p[1];
+    const int wb = ws[kb];
+    XQuarter<T> x[MT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int kb = min(k0 + u * KW, nb - 1);          // (behind the end: the last block once more, not used)
-      const i32x4* p = reinterpret_cast<const i32x4*>(wp + (int64_t)kb * 128);
-      lo[u] = p[0]; hi[u] = p[1];
-      wb[u] = ws[kb];
+    for (int j = 0; j < MT; ++j) x[j].load(a, m[j], kb, g);
+    const float sw = power_(wb);
+    bf16x8 fw[4];
+    expand_(lo, sw, fw);
+    expand_(hi, sw, fw + 2);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) x[u][j].load(a, m[j], kb, g);
-    }
+    for (int j = 0; j < MT; ++j) {
+      i32x4 q[2];
+      int byte;
+      x[j].values(q, byte);
+      const float sx = power_(byte);
+      bf16x8 fx[4];
+      expand_(q[0], sx, fx);
+      expand_(q[1], sx, fx + 2);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (k0 + u * KW >= nb) break;
-      const float sw = power_(wb[u]);
-      bf16x8 fw[4];
-      expand_(lo[u], sw, fw);
-      expand_(hi[u], sw, fw + 2);
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        i32x4 q[2];
-        int byte;
-        x[u][j].values(q, byte);
-        const float sx = power_(byte);
-        bf16x8 fx[4];
-        expand_(q[0], sx, fx);
-        expand_(q[1], sx, fx + 2);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[k], fx[k], acc[j], 0, 0, 0);
-      }
+      for (int k = 0; k < 4; ++k) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[k], fx[k], acc[j], 0, 0, 0);
     }
   }
 #pragma unroll
@@ -598,16 +589,8 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
 
 template <int T, int MT>
 void few_(const BlocksDenseArgs& a, hipStream_t st) {
-  constexpr int U = MT == 1 ? (T == BLOCKS_F32 ? 2 : 4) : MT == 2 && T != BLOCKS_F32 ? 2 : 1;
-  hipLaunchKernelGGL((dense_few_kernel<T, MT, U>), dim3((a.N + 15) / 16, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(512), 0, st, a);
+  hipLaunchKernelGGL((dense_few_kernel<T, MT>), dim3((a.N + 15) / 16, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(512), 0, st, a);
 }
-template <int T>
-void few_rows_(const BlocksDenseArgs& a, int mt, hipStream_t st) {
-  if (mt == 1) few_<T, 1>(a, st);
-  else if (mt == 2) few_<T, 2>(a, st);
-  else few_<T, 4>(a, st);
-}
-
 // Tiles of 16 rows per workgroup of the few-rows form, 0 where the tiled form is taken.  The former costs what its workgroups cost -- some 4.5 us up to 256 of
 // them, then in proportion -- and the more rows a workgroup has, the fewer times the weights are read; the latter has 15 us of latency at k = 2048
 // but does four times the work in a given time.  Measured at k = 2048, us for 1, 2, 4 tiles a workgroup | tiled: 64 x 2048 features 6.4, 5.8, 7.9 | 15.1;
@@ -668,40 +651,65 @@ void launch_blocks_dequantize(const BlocksDequantArgs& a, hipStream_t st) {
   }
 }
 
-// Rows that are not in blocks and go to the tiled form are quantised into the workspace first (the few-rows form quantises them on the way); y in
-// blocks from the few-rows form goes through f32 rows in the workspace, because its workgroups hold 16 of a block's 128 features.
+namespace {
+
+// How a call runs and what it keeps in the workspace: x in blocks where the product does not quantise it on the way, and y as f32 rows where it is wanted in
+// blocks from the few-rows form, whose workgroups hold 16 of a block's 128 features.
+struct Plan {
+  int mt = 0;                          // few_tiles_()
+  bool fused = false;                  // x is quantised by the few-rows form on the way: once for every 16 features
+  int64_t ldq = 0, lds = 0, ldy = 0;   // of x in blocks, of y in f32
+  size_t x_bytes = 0, y_bytes = 0;
+  // Quantising on the way saves a launch (some 3 us) and costs in proportion to rows x features / 16.  Measured, us on the way | first, f16 (f32) rows, k = 2048:
+  // 16 x 2048 5.8 | 7.1; 1009 x 29 5.7 | 7; 64 x 2048 9.6 (12.0) | 9.1 (9.4); 4000 x 29 (18.4) | (13.5): up to 256 workgroups of 16 rows.
+  Plan(int x_type, int y_type, int64_t M, int N, int K, int ordered) {
+    mt = ordered ? 0 : few_tiles_(M, N);
+    fused = x_type != BLOCKS_E4M3 && mt == 1 && (M + 15) / 16 * ((N + 15) / 16) <= 256;
+    if (x_type != BLOCKS_E4M3 && !fused) {
+      ldq = ((int64_t)K + 127) / 128 * 128; lds = ((int64_t)K + 511) / 512 * 4;
+      x_bytes = ((size_t)M * (ldq + lds) + 15) / 16 * 16;
+    }
+    if (mt && y_type == BLOCKS_E4M3) {
+      ldy = ((int64_t)N + 3) / 4 * 4;
+      y_bytes = (size_t)M * ldy * 4;
+    }
+  }
+};
+
+}  // namespace
+
 size_t blocks_dense_workspace(int x_type, int y_type, int64_t M, int N, int K, int ordered) {
   if (M < 1) return 0;
-  if (!ordered && few_tiles_(M, N)) return y_type == BLOCKS_E4M3 ? (size_t)M * (((size_t)N + 3) / 4 * 4) * 4 : 0;
-  return x_type == BLOCKS_E4M3 ? 0 : (size_t)M * (((size_t)K + 127) / 128 * 128 + ((size_t)K + 511) / 512 * 4);
+  const Plan p(x_type, y_type, M, N, K, ordered);
+  return p.x_bytes + p.y_bytes;
 }
 
 void launch_blocks_dense(const BlocksDenseArgs& args, void* workspace, hipStream_t st) {
   BlocksDenseArgs a = args;
   if (a.M < 1) return;
-  if (const int mt = a.ordered ? 0 : few_tiles_(a.M, a.N)) {
-    if (a.y_type == BLOCKS_E4M3) { a.y = workspace; a.y_type = BLOCKS_F32; a.ldy = ((int64_t)a.N + 3) / 4 * 4; a.vec = 1; }
-    switch (a.x_type) {
-      case BLOCKS_F32: few_rows_<BLOCKS_F32>(a, mt, st); break;
-      case BLOCKS_F16: few_rows_<BLOCKS_F16>(a, mt, st); break;
-      case BLOCKS_BF16: few_rows_<BLOCKS_BF16>(a, mt, st); break;
-      default: few_rows_<BLOCKS_E4M3>(a, mt, st); break;
-    }
-    if (args.y_type == BLOCKS_E4M3) {
+  const Plan p(a.x_type, a.y_type, a.M, a.N, a.K, a.ordered);
+  if (p.x_bytes) {
+    BlocksQuantArgs q{};
+    q.x = a.x; q.ldx = a.ldx; q.rows = a.M; q.cols = a.K; q.type = a.x_type; q.block_rows = 1; q.vec = a.xvec;
+    q.ldq = p.ldq; q.lds = p.lds; q.q = static_cast<unsigned char*>(workspace); q.scale = q.q + a.M * q.ldq;
+    launch_blocks_quantize(q, st);
+    a.x = q.q; a.x_scale = q.scale; a.ldx = q.ldq; a.ldxs = q.lds; a.x_type = BLOCKS_E4M3;
+  }
+  if (p.mt) {
+    if (p.y_bytes) { a.y = static_cast<unsigned char*>(workspace) + p.x_bytes; a.y_type = BLOCKS_F32; a.ldy = p.ldy; a.vec = 1; }
+    if (a.x_type == BLOCKS_F32) few_<BLOCKS_F32, 1>(a, st);
+    else if (a.x_type == BLOCKS_F16) few_<BLOCKS_F16, 1>(a, st);
+    else if (a.x_type == BLOCKS_BF16) few_<BLOCKS_BF16, 1>(a, st);
+    else if (p.mt == 1) few_<BLOCKS_E4M3, 1>(a, st);
+    else if (p.mt == 2) few_<BLOCKS_E4M3, 2>(a, st);
+    else few_<BLOCKS_E4M3, 4>(a, st);
+    if (p.y_bytes) {
       BlocksQuantArgs q{};
-      q.x = workspace; q.ldx = a.ldy; q.rows = a.M; q.cols = a.N; q.type = BLOCKS_F32; q.block_rows = 1; q.vec = 1;
+      q.x = a.y; q.ldx = a.ldy; q.rows = a.M; q.cols = a.N; q.type = BLOCKS_F32; q.block_rows = 1; q.vec = 1;
       q.q = static_cast<unsigned char*>(args.y); q.scale = args.y_scale; q.ldq = args.ldy; q.lds = args.ldys;
       launch_blocks_quantize(q, st);
     }
     return;
-  }
-  if (a.x_type != BLOCKS_E4M3) {
-    BlocksQuantArgs q{};
-    q.x = a.x; q.ldx = a.ldx; q.rows = a.M; q.cols = a.K; q.type = a.x_type; q.block_rows = 1; q.vec = a.xvec;
-    q.ldq = ((int64_t)a.K + 127) / 128 * 128; q.lds = ((int64_t)a.K + 511) / 512 * 4;
-    q.q = static_cast<unsigned char*>(workspace); q.scale = q.q + a.M * q.ldq;
-    launch_blocks_quantize(q, st);
-    a.x = q.q; a.x_scale = q.scale; a.ldx = q.ldq; a.ldxs = q.lds; a.x_type = BLOCKS_E4M3;
   }
   // Rows of a tile: larger tiles do more work for what they stage, smaller ones fill the chip sooner.  Measured at k = 2048, us for 64 / 128 / 256 rows:
   // 512 x 8192 features 24.9 / 26.7 / 37.7 and 2048 x 2048 26.0 / 27.1 / 37.7 (256 tiles of 128 rows); 1024 x 8192 43.7 / 39.6 / 40.9 and 6144 x 2048

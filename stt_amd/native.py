@@ -181,7 +181,7 @@ def lib():
         "STTX_ShardUtterances": (ci, [pp(cu), cu, cu, pp(cu)]),
         "STTX_QuantizeBlocks": (ci, [vp, ci, cl, cl, cl, ci, vp, cl, vp, cl, vp]),
         "STTX_DequantizeBlocks": (ci, [vp, cl, vp, cl, cl, cl, ci, vp, ci, cl, vp]),
-        "STTX_DenseBlocks": (ci, [pp(DenseBlocksArgs)]),
+        "STTX_DenseBlocks": (ci, [vp]),       # const STTX_DenseBlocksArgs*: byref(DenseBlocksArgs), or its bytes
         "STTX_DenseBlocksWorkspace": (C.c_ulonglong, [ci, ci, cl, cl, cl]),
         "STTX_TestFleetRecords": (pp(vp), [pp(cs), pp(cu), cu, cu]),
         "STTX_DebugFleetFailShard": (ci, [vp, ci]),

@@ -92,9 +92,15 @@ def test_workspace(L):
     assert W(3, 0, 1 << 20, 2048, 8192) == 0                  # already in blocks
     assert W(0, 1, 1, 2048, 2048) == 0                        # few rows are quantised on the way
     assert W(3, 3, 16, 2048, 2046) == 16 * 2048 * 4           # ... and their results, where those go on in blocks
+    assert W(1, 3, 100, 494, 2046) == (100 * (512 + 4) + 15) // 16 * 16 + 100 * 2048 * 4       # ... of a few more, both
     assert W(1, 0, 6144, 494, 2048) == 6144 * (512 + 4) == W(1, 3, 6144, 494, 2048)
     assert W(2, 2, 1 << 20, 130, 2048) == (1 << 20) * (256 + 4)
     assert W(9, 0, 100, 100, 100) == 0 and W(0, 0, -1, 100, 100) == 0 and W(0, -1, 5000, 100, 9000) == 0 and W(0, 0, 5000, 0, 9000) == 0
+
+
+def test_argument_block_is_the_structure():
+    v = tuple(range(1, 10)) + tuple(range(-6, 0)) + (77,) + (8, 9, 10) + (2, 3, 20.0)
+    assert blocks._ARGS(*v) == bytes(native.DenseBlocksArgs(*v)) and C.sizeof(native.DenseBlocksArgs) == len(blocks._ARGS(*v))
 
 
 def test_python_refuses():
