@@ -17,13 +17,14 @@ LIB = os.path.join(HERE, "lib", "libstt.so")
 LIB_TEST = os.path.join(HERE, "lib", "libstt_test.so")
 HOOK_SOURCES = ["kernels_am.hip", "kernels_i8.hip", "ctc.hip", "api.cpp", "fleet.cpp"]
 SOURCES = ["kernels_am.hip", "kernels_i8.hip", "kernels_blocks.hip", "ctc.hip", "hostutil.cpp", "scorer_dev.cpp", "model.cpp", "tflite_reader.cpp", "engine.cpp", "api.cpp", "blocks.cpp", "fleet.cpp"]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-x", "hip", "-Wno-unused-result"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-x", "hip", "-Wno-unused-result",
+         # float arithmetic one value an instruction: some packed f32 forms have given wrong results on this hardware now and then
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # ctc.hip: the search kernels run 1024 threads per workgroup (128 registers per lane) through one very long timestep loop.  Machine-level
 # loop-invariant code motion hoists every `thread index * 4 + LDS constant` address and every f64 polynomial coefficient of the bit-exact
 # logf / expf out of that loop and then SPILLS them (scratch loads where one v_add / two v_mov would do): 41 spilled vector registers
 # with it, none without (benchmarks/kernel_resources.sh).
-# kernels_blocks.hip: float arithmetic one value an instruction (some packed f32 forms have given wrong results on this hardware now and then).
-EXTRA_FLAGS = {"ctc.hip": ["-mllvm", "-disable-machine-licm"], "kernels_blocks.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
+EXTRA_FLAGS = {"ctc.hip": ["-mllvm", "-disable-machine-licm"]}
 
 
 def _newer(a, b):
