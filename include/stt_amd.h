@@ -189,7 +189,8 @@ STTX_EXPORT int STTX_QuantizeBlocks(const void* aX, int aType, long long aRows, 
 STTX_EXPORT int STTX_DequantizeBlocks(const unsigned char* aQ, long long aLdQ, const unsigned char* aScale, long long aLdScale, long long aRows,
                                      long long aCols, int aBlockRows, void* aY, int aType, long long aLdY, void* aStream);
 /* A dense layer: y[m][n] = epi(sum over k of x[m][k] * w[n][k] + bias[n]), sums in 32 bits; epi is nothing, or (relu_clip > 0) the graph's clipped
- * ReLU min(max(y, 0), relu_clip) -- NaN stays NaN.  Operands count as float32 holds them: beyond its range (scale bytes above 247) they are
+ * ReLU min(max(y, 0), relu_clip) -- NaN stays NaN.  The same call gives the same bits every time; beside another number of rows a row's sum may run in
+ * another order (its last bits).  Operands count as float32 holds them: beyond its range (scale bytes above 247) they are
  * infinities; magnitudes below 2^-126 may count as zero. */
 typedef struct STTX_DenseBlocksArgs {
   const void* x;                    /* [rows][in]: in blocks of 1 x 128 (x_type STTX_E4M3, x_scale), or f32 / f16 / bf16, quantised so by the call */

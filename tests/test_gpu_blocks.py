@@ -265,6 +265,18 @@ def test_rows_far_apart():
         del big, x, far, fb
 
 
+def test_more_rows_than_one_grid_dimension_has_threads():
+    """2^26 + 5 rows (a wave each: 2^32 threads and more): every row quantised, read back and multiplied, the last ones too."""
+    rows = (1 << 26) + 5
+    x = (torch.arange(rows, device="cuda", dtype=torch.int32) % 15 + 1).to(torch.float16)[:, None]       # 1 .. 15: whole numbers e4m3 holds
+    b = blocks.quantize_blocks(x)
+    y = blocks.dequantize_blocks(b, torch.float16)
+    assert torch.equal(x, y)
+    del y
+    w = blocks.quantize_blocks(torch.full((1, 1), 2.0, device="cuda"), 128)
+    assert torch.equal(blocks.dense_blocks(b, w, dtype=torch.float16), 2 * x)
+
+
 def _stack(x, layers, dtype):
     for w, b in layers[:-1]:
         x = blocks.dense_blocks(x, w, b, relu_clip=20.0, dtype=E4M3)
