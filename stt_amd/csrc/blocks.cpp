@@ -137,7 +137,7 @@ int STTX_DenseBlocks(const STTX_DenseBlocksArgs* aArgs) {
     a.M = c.rows; a.ldx = c.x_ld; a.ldxs = c.x_scale_ld; a.ldw = c.w_ld; a.ldws = c.w_scale_ld; a.ldy = c.y_ld; a.ldys = c.y_scale_ld;
     a.N = (int)c.out; a.K = (int)c.in; a.x_type = c.x_type; a.y_type = c.y_type; a.relu = c.relu_clip > 0.0f; a.clip = c.relu_clip;
     if (c.x_type != STTX_E4M3) a.xvec = vec16(c.x, c.x_type, c.x_ld);
-    if (c.y_type != STTX_E4M3) a.vec = aligned(c.y, 4 * elem(c.y_type)) && c.y_ld % 4 == 0;
+    if (c.y_type != STTX_E4M3) { a.vec = aligned(c.y, 4 * elem(c.y_type)) && c.y_ld % 4 == 0; a.wide = vec16(c.y, c.y_type, c.y_ld); }
     launch_blocks_dense(a, c.workspace, st);
     HIP_CHECK(hipGetLastError());
   });

@@ -122,7 +122,7 @@ static void f8_dense(const ModelState::BlocksMatrix& w, const float* bias, const
   if (x_type == BLOCKS_E4M3) { a.ldx = blocks_ld(w.K); a.ldxs = blocks_lds(w.K); a.x_scale = static_cast<const unsigned char*>(x) + M * a.ldx; }
   else a.xvec = ldx % 8 == 0;
   a.w = w.values.as<unsigned char>(); a.w_scale = w.scale.as<unsigned char>(); a.ldw = blocks_ld(w.K); a.ldws = blocks_lds(w.K);
-  a.bias = bias; a.y = y; a.y_type = y_type; a.ldy = w.N; a.vec = w.N % 4 == 0;
+  a.bias = bias; a.y = y; a.y_type = y_type; a.ldy = w.N; a.vec = w.N % 4 == 0; a.wide = w.N % 8 == 0;
   if (y_type == BLOCKS_E4M3) { a.ldy = blocks_ld(w.N); a.ldys = blocks_lds(w.N); a.y_scale = static_cast<unsigned char*>(y) + M * a.ldy; }
   a.relu = clip > 0.0f; a.clip = clip; a.lds_floor = lds_floor;
   a.ordered = 1;      // transcripts do not depend on how utterances and streams were grouped

@@ -162,7 +162,7 @@ struct BlocksDenseArgs {
   int N, K, x_type, y_type, relu;
   float clip;
   int xvec;                 // rows of an f32 / f16 / bf16 x may be read 16 bytes at a time
-  int vec;                  // rows of y may be written four values at a time
+  int vec, wide;            // rows of an f32 / f16 / bf16 y may be written four values, 16 bytes at a time
   int ordered;              // 1: every sum runs along k in ONE order however many rows there are (the tiled form always): a row's results do not depend on the rows beside it
   int lds_floor;            // as DenseArgs::lds_floor
 };

@@ -367,47 +367,89 @@ __global__ __launch_bounds__(512) void dense_few_kernel(BlocksDenseArgs a) {
   }
 }
 
-// The results of a wave that holds the features n0 + no .. of a block of 128, 16 NI of them, in the rows m, m + 16 .. (m the lane's own): acc[i][j][r] is feature
-// n0 + no + 16 i + 4 g + r of row m + 16 j.  bias: the block's 128 biases in LDS.  A row's largest value in blocks is the largest of WN waves' (tops,
-// in LDS: [WN][rows of the workgroup], row `ml` the lane's first).
-template <int NI, int MJ, int WN, int BM, int Y>
-__device__ __forceinline__ void tile_results_as_(const BlocksDenseArgs& a, f32x4 (&acc)[NI][MJ], int64_t m, int ml, int n0, int no, int g, const float* bias, unsigned* tops) {
-  const bool whole = n0 + 128 <= a.N && (Y == BLOCKS_E4M3 || a.vec != 0);
+// Sixteen rows of a wave's results in 8 or 16 bits through LDS (its own part of it), so that they leave 16 bytes a lane along a row: straight from the
+// accumulators a store writes an eighth to a quarter of a line in each of sixteen rows.  Measured, us straight | through LDS: 6144 x 2048 features in blocks
+// 53.1 | 49.9, 6144 x 8192 f16 174 | 171; f32, half a line a row and store, is better off straight (2048 x 8192 61.2 | 65.8).
+// Lane (li, g) holds 4 values = `Q` bytes at feature 16 i + 4 g of row li.
+template <int NI, int Q> struct RowsOut {
+  static constexpr int BYTES = NI * 4 * Q, PITCH = BYTES + 16, CHUNKS = BYTES / 16;      // of a row; the pitch keeps a column's rows on different banks
+  lds_u8* buf;
+  int li, g, lane;
+  template <class V> __device__ __forceinline__ void put(int i, V v) {
+    static_assert(sizeof(V) == Q, "four values");
+    *reinterpret_cast<__attribute__((address_space(3))) V*>(buf + li * PITCH + (i * 4 + g) * Q) = v;
+  }
+  // row r of the sixteen goes to y + r * ld, rows < `rows`
+  __device__ __forceinline__ void leave(unsigned char* y, int64_t ld, int64_t rows) {
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int n = n0 + no + i * 16 + g * 4;
-    const f32x4 b = *reinterpret_cast<const f32x4*>(bias + no + i * 16 + g * 4);
-#pragma unroll
-    for (int j = 0; j < MJ; ++j) {
-      f32x4 v = acc[i][j] + b;
-      if (a.relu) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = epi_(v[r], true, a.clip);
-      }
-      if constexpr (Y == BLOCKS_E4M3) {
-        acc[i][j] = v;
-        if (!whole) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] = n + r < a.N ? v[r] : 0.0f;
-        }
-      } else if (m + j * 16 < a.M) {
-        typename Elem<Y>::type* y = reinterpret_cast<typename Elem<Y>::type*>(a.y) + (m + j * 16) * a.ldy + n;
-        if (whole) {
-          if constexpr (Y == BLOCKS_F32) *reinterpret_cast<f32x4*>(y) = v;
-          else {
-            u16x4 o;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = Y == BLOCKS_BF16 ? f32_bf16(v[r]) : __builtin_bit_cast(unsigned short, (_Float16)v[r]);
-            *reinterpret_cast<u16x4*>(y) = o;
-          }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) if (n + r < a.N) store1<Y>(y + r, v[r]);
-        }
-      }
+    for (int t = 0; t < 16 * CHUNKS / 64; ++t) {
+      const int idx = t * 64 + lane, r = idx / CHUNKS, c = idx % CHUNKS;
+      const i32x4 v = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(buf + r * PITCH + c * 16);
+      if (r < rows) *reinterpret_cast<i32x4*>(y + r * ld + c * 16) = v;
     }
   }
-  if constexpr (Y == BLOCKS_E4M3) {
+};
+
+// The results of a wave that holds the features n0 + no .. of a block of 128, 16 NI of them, in the rows m0 + 16 j + li: acc[i][j][r] is feature
+// n0 + no + 16 i + 4 g + r of row m0 + 16 j + li.  bias: the block's 128 biases in LDS.  A row's largest value in blocks is the largest of WN waves'
+// (tops, in LDS: [WN][rows of the workgroup], row `ml` the lane's first).  buf: this wave's 16 * 272 bytes of LDS.
+template <int NI, int MJ, int WN, int BM, int Y>
+__device__ __forceinline__ void tile_results_as_(const BlocksDenseArgs& a, f32x4 (&acc)[NI][MJ], int64_t m0, int ml, int n0, int no, int lane, const float* bias, unsigned* tops, lds_u8* buf) {
+  const int li = lane & 15, g = lane >> 4;
+  const int64_t m = m0 + li;
+  const bool whole = n0 + 128 <= a.N && (Y == BLOCKS_E4M3 || a.wide != 0);
+  auto result = [&](int i, int j) {
+    f32x4 v = acc[i][j] + *reinterpret_cast<const f32x4*>(bias + no + i * 16 + g * 4);
+    if (a.relu) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = epi_(v[r], true, a.clip);
+    }
+    return v;
+  };
+  if constexpr (Y != BLOCKS_E4M3) {
+    typedef typename Elem<Y>::type elem;
+    if (Y != BLOCKS_F32 && whole) {
+      RowsOut<NI, 8> out{buf, li, g, lane};
+#pragma unroll
+      for (int j = 0; j < MJ; ++j) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const f32x4 v = result(i, j);
+          u16x4 o;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[r] = Y == BLOCKS_BF16 ? f32_bf16(v[r]) : __builtin_bit_cast(unsigned short, (_Float16)v[r]);
+          out.put(i, o);
+        }
+        out.leave(reinterpret_cast<unsigned char*>(a.y) + ((m0 + j * 16) * a.ldy + n0 + no) * 2, a.ldy * 2, a.M - (m0 + j * 16));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < MJ; ++j) {
+          const f32x4 v = result(i, j);
+          const int n = n0 + no + i * 16 + g * 4;
+          elem* const y = reinterpret_cast<elem*>(a.y) + (m + j * 16) * a.ldy + n;
+          if (m + j * 16 < a.M) {
+            if (Y == BLOCKS_F32 && whole) *reinterpret_cast<f32x4*>(y) = v;
+            else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) if (n + r < a.N) store1<Y>(y + r, v[r]);
+            }
+          }
+        }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < MJ; ++j) {
+        acc[i][j] = result(i, j);
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] = n0 + no + i * 16 + g * 4 + r < a.N ? acc[i][j][r] : 0.0f;
+        }
+      }
     unsigned top[MJ];
     auto row_tops = [&](bool all) {
 #pragma unroll
@@ -437,20 +479,19 @@ __device__ __forceinline__ void tile_results_as_(const BlocksDenseArgs& a, f32x4
 #pragma unroll
         for (int w = 0; w < WN; ++w) top[j] = max(top[j], tops[w * BM + ml + j * 16]);
     }
+    RowsOut<NI, 4> out{buf, li, g, lane};
 #pragma unroll
     for (int j = 0; j < MJ; ++j) {
       const int byte = scale_byte_(top[j]);
       const float power = power_(byte);
-      if (m + j * 16 < a.M) {
-        unsigned char* y = reinterpret_cast<unsigned char*>(a.y) + (m + j * 16) * a.ldy + n0 + no + g * 4;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) *reinterpret_cast<unsigned*>(y + i * 16) = pack4_(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], power);
-        if (no == 0) {
-          const int b = n0 >> 7, last = ((a.N + 127) >> 7) - 1, pad = ((last + 4) & ~3) - 1;
-          unsigned char* ys = a.y_scale + (m + j * 16) * a.ldys + b;
-          if (g == 0) ys[0] = (unsigned char)byte;
-          if (b == last && g > 0 && b + g <= pad) ys[g] = kUnit;
-        }
+      for (int i = 0; i < NI; ++i) out.put(i, pack4_(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], power));
+      out.leave(reinterpret_cast<unsigned char*>(a.y) + (m0 + j * 16) * a.ldy + n0 + no, a.ldy, a.M - (m0 + j * 16));
+      if (no == 0 && m + j * 16 < a.M) {
+        const int blk = n0 >> 7, last = ((a.N + 127) >> 7) - 1, pad = ((last + 4) & ~3) - 1;
+        unsigned char* ys = a.y_scale + (m + j * 16) * a.ldys + blk;
+        if (g == 0) ys[0] = (unsigned char)byte;
+        if (blk == last && g > 0 && blk + g <= pad) ys[g] = kUnit;
       }
     }
   }
@@ -580,13 +621,15 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
   BLOCKS_ARRIVE(0);
   step(cur);
 #undef BLOCKS_ARRIVE
-  const int64_t m = m0 + wm * MJ * 16 + li;
+  if (a.y_type != BLOCKS_F32) __syncthreads();      // every wave is done reading the stages: LDS is the results' now
+  const int64_t mw = m0 + wm * MJ * 16;
   const int ml = wm * MJ * 16 + li, no = wn * NI * 16;
+  lds_u8* const buf = lds + wave * (16 * 272);
   switch (a.y_type) {
-    case BLOCKS_F32: tile_results_as_<NI, MJ, WN, BM, BLOCKS_F32>(a, acc, m, ml, n0, no, g, s_bias, s_tops); break;
-    case BLOCKS_F16: tile_results_as_<NI, MJ, WN, BM, BLOCKS_F16>(a, acc, m, ml, n0, no, g, s_bias, s_tops); break;
-    case BLOCKS_BF16: tile_results_as_<NI, MJ, WN, BM, BLOCKS_BF16>(a, acc, m, ml, n0, no, g, s_bias, s_tops); break;
-    default: tile_results_as_<NI, MJ, WN, BM, BLOCKS_E4M3>(a, acc, m, ml, n0, no, g, s_bias, s_tops); break;
+    case BLOCKS_F32: tile_results_as_<NI, MJ, WN, BM, BLOCKS_F32>(a, acc, mw, ml, n0, no, lane, s_bias, s_tops, buf); break;
+    case BLOCKS_F16: tile_results_as_<NI, MJ, WN, BM, BLOCKS_F16>(a, acc, mw, ml, n0, no, lane, s_bias, s_tops, buf); break;
+    case BLOCKS_BF16: tile_results_as_<NI, MJ, WN, BM, BLOCKS_BF16>(a, acc, mw, ml, n0, no, lane, s_bias, s_tops, buf); break;
+    default: tile_results_as_<NI, MJ, WN, BM, BLOCKS_E4M3>(a, acc, mw, ml, n0, no, lane, s_bias, s_tops, buf); break;
   }
 }
 
