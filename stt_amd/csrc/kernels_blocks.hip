@@ -497,9 +497,13 @@ __device__ __forceinline__ void tile_results_as_(const BlocksDenseArgs& a, f32x4
   }
 }
 
-// Many rows: 128 features by BM rows per workgroup of four waves, WN of them along the features.  Both operands are staged as
-// e4m3 through LDS by global_load_lds, 64 values along k a step and three stages: two steps in flight behind a counted wait.  A staged row
-// is 64 bytes, its 16-byte chunk c at slot c ^ (row bit 3) * 2, which keeps the sixteen lanes a ds_read_b128 is serviced in on different banks.
+// Many rows: 128 features by BM rows per workgroup of four waves, WN of them along the features.  Both operands are staged as e4m3 through LDS by
+// global_load_lds, 64 values along k a step and three stages: two steps in flight behind a counted wait, half the LDS traffic of staged bf16.  A staged
+// row is 64 bytes, its 16-byte chunk c at slot c ^ (row bit 3) * 2, which keeps the sixteen lanes a ds_read_b128 is serviced in on different banks.
+// A wave of the 256-row tile turns 12 fragments into bf16 for 64 products a step (96 conversions, which the other workgroup's products hide);
+// two such workgroups fit a compute unit, three of the 128-row tile.  32000 x 8192 x 2048 to f32: 927 us = 1158 TFLOP/s, the matrix cores busy 56 % of the
+// time; a library's bf16 product of that shape takes 919 us and writes half as much.  The clock falls with the data (the same call on
+// operands of all ones: 13 % less): power, not one unit, is what is left.
 template <int BM, int WN>
 __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
   constexpr int BN = 128, WM = 4 / WN, NI = 8 / WN, MJ = BM / 16 / WM;
@@ -644,14 +648,18 @@ template <int T, int MT>
 void few_(const BlocksDenseArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((dense_few_kernel<T, MT>), dim3((a.N + 15) / 16, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(512), 0, st, a);
 }
-// Tiles of 16 rows per workgroup of the few-rows form, 0 where the tiled form is taken.  The former costs what its workgroups cost -- some 4.5 us up to 256 of
-// them, then in proportion -- and the more rows a workgroup has, the fewer times the weights are read; the latter has 15 us of latency at k = 2048
-// but does four times the work in a given time.  Measured at k = 2048, us for 1, 2, 4 tiles a workgroup | tiled: 64 x 2048 features 6.4, 5.8, 7.9 | 15.1;
-// 32 x 8192 10.7, 9.1, 10.8 | 15; 128 x 2048 10.6, 9.0, 8.1 | 15.2; 256 x 2048 18.6, 15.4, 13.9 | 15.3; 128 x 8192 34, 28, 25 | 15.8.
+// Tiles of 16 rows per workgroup of the few-rows form, 0 where the tiled form is taken.  The former costs what its workgroups cost -- some 4.2 us up to 256 of
+// them, then in proportion -- and more rows a workgroup read the weights fewer times; the latter takes 14.5 us at k = 2048 for the latency of its steps,
+// but does four times the work in a given time.  So: the fewest rows that need at most 256 workgroups, or as many as there are where those need at
+// most 512.  Measured at k = 2048, us for 1, 2, 4 tiles a workgroup | tiled: 32 x 2048 features 4.2, 5.4, 6.4 | 14.6; 64 x 2048 6.2, 5.5, 7.7 | 14.9; 16 x 8192
+// 6.1, 6.8, 8.2 | 14.3; 32 x 8192 10.3, 8.5, 9.9 | 14.8; 128 x 2048 10.2, 8.6, 7.8 | 15.0; 256 x 2048 18.3, 15.0, 13.2 | 15.0; 512 x 2048 34, 27, 25 | 15.4.
 int few_tiles_(int64_t M, int N) {
   const int64_t n = (N + 15) / 16;
-  for (int mt = 1; mt <= 4; mt *= 2) if ((M + 16 * mt - 1) / (16 * mt) * n <= 512) return mt;
-  return 0;
+  for (int mt = 1;; mt *= 2) {
+    const int64_t groups = (M + 16 * mt - 1) / (16 * mt) * n;
+    if (groups <= 256) return mt;
+    if (mt == 4 || M <= 16 * mt) return groups <= 512 ? mt : 0;
+  }
 }
 
 template <int BM, int WN>
@@ -761,9 +769,9 @@ void launch_blocks_dense(const BlocksDenseArgs& args, void* workspace, hipStream
     return;
   }
   // Rows of a tile: larger tiles do more work for what they stage, smaller ones fill the chip sooner.  Measured at k = 2048, us for 64 / 128 / 256 rows:
-  // 512 x 8192 features 24.9 / 26.7 / 37.7 and 2048 x 2048 26.0 / 27.1 / 37.7 (256 tiles of 128 rows); 1024 x 8192 43.7 / 39.6 / 40.9 and 6144 x 2048
-  // 63.9 / 55.4 / 59.1 (256 and 384 tiles of 256 rows: less than two workgroups for every compute unit); 2048 x 8192 81.5 / 72.1 / 65.2;
-  // 6144 x 8192 231 / 200 / 177; 32000 x 8192 1238 / 1056 / 1026.
+  // 512 x 8192 features 24.6 / 27.8 / 37.0 and 2048 x 2048 24.0 / 26.8 / 36.9 (256 tiles of 128 rows); 1024 x 8192 43.0 / 40.1 / 40.0 and 6144 x 2048
+  // in blocks 59.7 / 51.9 / 55.5 (256 and 384 tiles of 256 rows: less than two workgroups for every compute unit); 2048 x 8192 82.2 / 74.0 / 65.5;
+  // 6144 x 8192 f16 221 / 193 / 173; 32000 x 8192 1253 / 1068 / 981.
   const int64_t tiles_n = (a.N + 127) / 128;
   if (tiles_n * ((a.M + 127) / 128) <= 256) tile_<64, 2>(a, st);
   else if (tiles_n * ((a.M + 255) / 256) < 512) tile_<128, 1>(a, st);
