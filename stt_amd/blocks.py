@@ -7,7 +7,7 @@ tensors in HBM: 8-bit floating point (e4m3) with one power of two per block of 1
     f = dequantize_blocks(h, torch.float32)                         # a hidden layer's rows read back
 
 Calls enqueue on torch's current stream of the tensors' device and allocate with torch, so they can be captured into a graph like any torch
-call.  No compute happens in Python; there is no fallback for tensors elsewhere.
+call.  No compute happens in Python; there is no fallback for tensors elsewhere, and there are no gradients: results are detached.
 
 A call on a few rows is over in less time than a careless caller needs to make it, so the checks below are one expression each on the way that
 succeeds, and the messages are put together on the way that fails.
@@ -22,6 +22,7 @@ BLOCK = 128
 E4M3 = torch.float8_e4m3fn
 _PLAIN = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}            # STTX_ElementType
 _E4M3 = 3
+_CLIP_MIN, _CLIP_MAX = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max   # (as a float32 nothing below it may become 0: no ReLU)
 _UINT8 = torch.uint8
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _ARGS = struct.Struct("9Q6q1Q3q2if4x").pack                                  # native.DenseBlocksArgs as bytes: a third of the time of filling one in
@@ -152,8 +153,8 @@ def dense_blocks(x, w, bias=None, relu_clip=None, dtype=torch.float16):
         b_ptr = bias.data_ptr()
     clip = 0.0
     if relu_clip is not None:
-        if not relu_clip > 0.0:
-            raise ValueError("relu_clip: a positive number or None is wanted, got %r" % (relu_clip,))
+        if not _CLIP_MIN <= relu_clip <= _CLIP_MAX and relu_clip != float("inf"):
+            raise ValueError("relu_clip: a positive number of float32's normal range, inf or None is wanted, got %r" % (relu_clip,))
         clip = relu_clip
     L = _lib or _entry()
     if dtype is E4M3:

@@ -717,8 +717,8 @@ struct Plan {
   bool fused = false;                  // x is quantised by the few-rows form on the way: once for every 16 features
   int64_t ldq = 0, lds = 0, ldy = 0;   // of x in blocks, of y in f32
   size_t x_bytes = 0, y_bytes = 0;
-  // Quantising on the way saves a launch (some 3 us) and costs in proportion to rows x features / 16.  Measured, us on the way | first, f16 (f32) rows, k = 2048:
-  // 16 x 2048 5.8 | 7.1; 1009 x 29 5.7 | 7; 64 x 2048 9.6 (12.0) | 9.1 (9.4); 4000 x 29 (18.4) | (13.5): up to 256 workgroups of 16 rows.
+  // Quantising on the way saves a launch (some 3 us) and costs in proportion to rows x features / 16.  Measured, us on the way | first, k = 2048:
+  // 16 x 2048 5.8 | 7.1; 1009 x 29 5.7 | 7; 64 x 2048 f16 9.6 | 8.1; 4000 x 29 f32 18.4 | 15.4: up to 256 workgroups of 16 rows.
   Plan(int x_type, int y_type, int64_t M, int N, int K, int ordered) {
     mt = ordered ? 0 : few_tiles_(M, N);
     fused = x_type != BLOCKS_E4M3 && mt == 1 && (M + 15) / 16 * ((N + 15) / 16) <= 256;

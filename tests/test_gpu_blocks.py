@@ -356,3 +356,48 @@ def test_refuses_on_the_gpu():
     assert blocks.dense_blocks(x[:0], w, b).shape == (0, 100) and blocks.quantize_blocks(x[:0]).shape == (0, 300)
     assert blocks.dequantize_blocks(blocks.quantize_blocks(x[:0])).shape == (0, 300)
     assert blocks.dense_blocks(x[:0], w, b, dtype=E4M3).shape == (0, 100)
+
+
+def test_clip_has_to_be_a_float32():
+    """A clip that float32 rounds to 0 would be no ReLU at all."""
+    w = blocks.quantize_blocks(torch.eye(4, device="cuda"), 128)
+    x = torch.tensor([[-4.0, 0.5, 8.0, 448.0]], device="cuda")
+    for clip in (1e-50, 1e-39, 1e39, -1.0, -float("inf")):
+        with pytest.raises(ValueError):
+            blocks.dense_blocks(x, w, relu_clip=clip)
+    assert host(blocks.dense_blocks(x, w, relu_clip=float("inf"), dtype=torch.float32)).tolist() == [[0.0, 0.5, 8.0, 448.0]]
+    assert host(blocks.dense_blocks(x, w, relu_clip=torch.finfo(torch.float32).tiny, dtype=torch.float32)).tolist() == [[0.0] + 3 * [float(torch.finfo(torch.float32).tiny)]]
+
+
+def test_threads():
+    """Calls from four threads at once, each on a stream of its own, all forms: every thread has its own results."""
+    import threading
+    rng = np.random.default_rng(12)
+    layers = _layers(rng, [494, 300, 100])
+    ops = [(w, b) for w, b, _ in layers]
+    sizes = (1, 16, 200, 5000)
+    data = [rng.integers(-8, 9, (m, 494)).astype(float) for m in sizes]
+    wants = [_stack_ref(xd, layers) for xd in data]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                x = torch.from_numpy(data[i]).half().cuda()
+                ys = [_stack(x, ops, torch.float32) for _ in range(20)]
+            s.synchronize()
+            got[i] = [host(y) for y in ys]
+        except Exception as e:                    # told by the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i, want in enumerate(wants):
+        for y in got[i]:
+            np.testing.assert_array_equal(y, want)
