@@ -1,6 +1,6 @@
 // stt_amd/csrc/tuning.h -- the engine's tunables in ONE table (internal header).
 //
-// Every value has a measured default; nothing here changes results, only what runs beside what
+// Every value has a measured default; nothing here but the choice of arithmetic (am_i8, am_f8) changes results, only what runs beside what
 // and which of several bit-identical kernel forms is launched.  Two ways in, both for A/B runs and tests:
 //   STTX_SetTuning("name", value)        between calls, nothing in flight (include/stt_amd.h)
 //   STT_AMD_TUNING="name=value,name=value"   read once, when the table is first used
