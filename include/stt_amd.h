@@ -252,7 +252,7 @@ typedef struct STTX_ModelInfo {
   float relu_clip;
   unsigned int alphabet_bytes;
   int is_tflite;
-  int hybrid_int8;                 /* 1: the file's six matrices are symmetric int8 and the model will run TFLite's hybrid arithmetic (STTX_GetAcousticMode 1) */
+  int hybrid_int8;                 /* 1: the file's six matrices are symmetric int8 and the model will run TFLite's hybrid arithmetic (STTX_GetAcousticMode 1; tunables am_i8, am_f8 aside) */
   int asymmetric_quantize_inputs;  /* 1: a FULLY_CONNECTED asks for asymmetric input quantisation: not restated, the weights are de-quantised (f16 path) */
 } STTX_ModelInfo;
 STTX_EXPORT int STTX_InspectModel(const char* aModelBuffer, unsigned int aBufferSize, STTX_ModelInfo* aInfo);

@@ -321,7 +321,7 @@ class Model(object):
         return probs, nc, nh
 
     def acousticMode(self):
-        """0 = f16 MFMA operands / f32 accumulate, 1 = TFLite's hybrid int8 arithmetic end to end (include/stt_amd.h: STTX_GetAcousticMode)."""
+        """0 = f16 MFMA operands / f32 accumulate, 1 = TFLite's hybrid int8 arithmetic end to end, 2 = dense layers in 8-bit floating point in blocks, the rest as in 0 (include/stt_amd.h: STTX_GetAcousticMode)."""
         return int(native.lib().STTX_GetAcousticMode(self._impl))
 
     def slowRows(self):

@@ -401,3 +401,20 @@ def test_threads():
     for i, want in enumerate(wants):
         for y in got[i]:
             np.testing.assert_array_equal(y, want)
+
+
+@pytest.mark.parametrize("m", [3, 40, 700])
+def test_parts_of_block_tensors(m):
+    """Rows out of the middle of a BlockTensor, features from a row of blocks on, fewer columns than the values have room for; results are detached."""
+    rng = np.random.default_rng(m)
+    xb, xd = whole_blocks(rng, m + 9, 300, 1)
+    wb, wd = whole_blocks(rng, 400, 300, 128)
+    x = blocks.BlockTensor(xb.values[4:4 + m], xb.scale[4:4 + m], 300)
+    w = blocks.BlockTensor(wb.values[128:], wb.scale[1:], 300, 128)
+    np.testing.assert_array_equal(host(blocks.dense_blocks(x, w, dtype=torch.float32)), R.dense(xd[4:4 + m], wd[128:]))
+    np.testing.assert_array_equal(host(blocks.dequantize_blocks(x)), xd[4:4 + m])
+    x1 = blocks.BlockTensor(x.values, x.scale, 256)                          # the first two blocks of a row
+    w1 = blocks.BlockTensor(w.values, w.scale, 256, 128)
+    np.testing.assert_array_equal(host(blocks.dense_blocks(x1, w1, dtype=torch.float32)), R.dense(xd[4:4 + m, :256], wd[128:, :256]))
+    p = torch.ones(4, 300, device="cuda", requires_grad=True)
+    assert not blocks.dense_blocks(p, w, dtype=torch.float32).requires_grad and not blocks.dequantize_blocks(blocks.quantize_blocks(p)).requires_grad
