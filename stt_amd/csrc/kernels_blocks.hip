@@ -20,6 +20,7 @@
 
 #include <mutex>
 #include <stdexcept>
+#include <type_traits>
 
 #include "kernels.h"
 
@@ -382,8 +383,9 @@ template <int NI, int Q> struct RowsOut {
   // row r of the sixteen goes to y + r * ld, rows < `rows`
   __device__ __forceinline__ void leave(unsigned char* y, int64_t ld, int64_t rows) {
 #pragma unroll
-    for (int t = 0; t < 16 * CHUNKS / 64; ++t) {
+    for (int t = 0; t < (16 * CHUNKS + 63) / 64; ++t) {
       const int idx = t * 64 + lane, r = idx / CHUNKS, c = idx % CHUNKS;
+      if (CHUNKS < 4 && r >= 16) break;
       const i32x4 v = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(buf + r * PITCH + c * 16);
       if (r < rows) *reinterpret_cast<i32x4*>(y + r * ld + c * 16) = v;
     }
@@ -498,20 +500,24 @@ __device__ __forceinline__ void tile_results_as_(const BlocksDenseArgs& a, f32x4
 }
 
 // Many rows: 128 features by BM rows per workgroup of four waves, WN of them along the features.  Both operands are staged as e4m3 through LDS by
-// global_load_lds, 64 values along k a step and three stages: two steps in flight behind a counted wait, half the LDS traffic of staged bf16.  A staged
-// row is 64 bytes, its 16-byte chunk c at slot c ^ (row bit 3) * 2, which keeps the sixteen lanes a ds_read_b128 is serviced in on different banks.
-// A wave of the 256-row tile turns 12 fragments into bf16 for 64 products a step (96 conversions, which the other workgroup's products hide);
-// two such workgroups fit a compute unit, three of the 128-row tile.  32000 x 8192 x 2048 to f32: 927 us = 1158 TFLOP/s, the matrix cores busy 56 % of the
-// time; a library's bf16 product of that shape takes 919 us and writes half as much.  The clock falls with the data (the same call on
-// operands of all ones: 13 % less): power, not one unit, is what is left.
-template <int BM, int WN>
+// global_load_lds, KS = 64 or 128 values along k a step and STAGES = 3 stages: two steps in flight behind a counted wait, half the LDS traffic of staged
+// bf16; the scale words of four blocks along k go the same way.  The 16-byte chunks of a staged row are permuted so that the sixteen lanes a ds_read_b128 is
+// serviced in are on different banks: chunk c of a 64-byte row r at slot c ^ (row bit 3) * 2, of a 128-byte row at c ^ (r / 2 mod 8).
+// Large tiles: a wave of the 256-row tile turns 12 fragments into bf16 for 64 products a step of 64 (96 conversions, which the other workgroup's
+// products hide); two such workgroups fit a compute unit, three of the 128-row tile.  32000 x 8192 x 2048 to f32: 914 us = 1175 TFLOP/s, the matrix cores
+// busy 56 % of the time; a library's bf16 product of that shape takes 919 us and writes half as much.  The clock falls with the data (the same
+// call on operands of all ones: 13 % less): power, not one unit, is what is left.
+// Small tiles: one wave a SIMD unit, so a step's latencies -- barrier, LDS, conversion, product -- add up, and more stages in flight change nothing (64
+// rows, 64 values a step, 3 / 5 / 7 stages: 15.6 / 15.1 / 15.0 us at k = 2048): 128 values a step halve the barriers (14.4) and 32 rows the work (11.3).
+template <int BM, int WN, int STAGES, int KS>
 __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
   constexpr int BN = 128, WM = 4 / WN, NI = 8 / WN, MJ = BM / 16 / WM;
-  constexpr int STAGE = (BN + BM) * 64, ITS = (BN + BM) / 64;      // a staging instruction of a wave covers sixteen rows
+  constexpr int STAGE = (BN + BM) * KS, XROWS = BM < 64 ? 64 : BM, SCALES = (XROWS + 64) * 4, SUB = 128 / KS, AHEAD = (STAGES - 1) / SUB;
+  constexpr int RPI = 1024 / KS, ITS = (BN + BM) / RPI / 4;      // a staging instruction of a wave covers sixteen rows
   __shared__ __attribute__((aligned(16))) float s_bias[BN];
   __shared__ unsigned s_tops[WN == 1 ? 1 : WN * BM];
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds_blocks[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, g = lane >> 4;
   const int wn = wave % WN, wm = wave / WN;
   lds_u8* const lds = (lds_u8*)lds_blocks;
   const int tiles_n = (a.N + BN - 1) / BN;
@@ -519,24 +525,24 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
   int64_t tile_m;
   {  // workgroup i runs on XCD i % 8: every XCD takes a run of tiles, 1024 rows at a time over all features, so that what it works on at once shares rows and
      // features (32000 x 8192 x 2048: 995 us with 1024 rows, 1009 and 1038 with 512 and 2048)
-    constexpr int GM = 1024 / BM;
-    const int64_t tiles_m = (a.M + BM - 1) / BM, total = tiles_n * tiles_m, per = (total + 7) / 8;
-    const int64_t idx = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    constexpr unsigned GM = 1024 / BM;      // (less than 2^24 tiles: checked on the host)
+    const unsigned tn = (unsigned)tiles_n, tiles_m = (unsigned)((a.M + BM - 1) / BM), total = tn * tiles_m, per = (total + 7) / 8;
+    const unsigned idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((blockIdx.x >> 3) >= per || idx >= total) return;
-    const int64_t first = idx / (GM * (int64_t)tiles_n) * GM;
-    const int high = (int)min(tiles_m - first, (int64_t)GM), rem = (int)(idx - first * tiles_n);
-    tile_n = rem / high;
+    const unsigned first = idx / (GM * tn) * GM, high = min(tiles_m - first, GM), rem = idx - first * tn;
+    tile_n = (int)(rem / high);
     tile_m = first + rem % high;
   }
   const int n0 = tile_n * BN;
   const int64_t m0 = tile_m * BM;
   if (tid < BN) s_bias[tid] = a.bias && n0 + tid < a.N ? a.bias[n0 + tid] : 0.0f;      // (visible behind the first barrier below)
   const int nb = (a.K + 127) >> 7;
+  auto swizzle = [](int r) { return KS == 64 ? ((r >> 3) & 1) << 1 : (r >> 1) & 7; };
   const unsigned char* src[ITS];
 #pragma unroll
   for (int i = 0; i < ITS; ++i) {
-    const int r = (wave + 4 * i) * 16 + (lane >> 2), c = (lane & 3) ^ (((r >> 3) & 1) << 1);      // rows 0 .. 127: w, then x
-    if (4 * i < BN / 16) src[i] = a.w + (int64_t)min(n0 + r, a.N - 1) * a.ldw + c * 16;
+    const int r = (wave + 4 * i) * RPI + lane / (KS / 16), c = (lane & (KS / 16 - 1)) ^ swizzle(r);      // rows 0 .. 127: w, then x
+    if (4 * i < BN / RPI) src[i] = a.w + (int64_t)min(n0 + r, a.N - 1) * a.ldw + c * 16;
     else {
       int64_t m = m0 + (r - BN);
       m = m < a.M ? m : a.M - 1;
@@ -547,18 +553,23 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
 #pragma unroll
     for (int i = 0; i < ITS; ++i) {
       __builtin_amdgcn_global_load_lds((gvoid_c*)src[i], (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (wave + 4 * i) * 1024), 16, 0, 0);
-      src[i] += 64;
+      src[i] += KS;
     }
   };
-  const unsigned char* xs[MJ];
-#pragma unroll
-  for (int j = 0; j < MJ; ++j) {
-    int64_t m = m0 + (wm * MJ + j) * 16 + li;
-    m = m < a.M ? m : a.M - 1;
-    xs[j] = a.x_scale + m * a.ldxs;
+  // the scale bytes of four blocks along k at a time: a word per row of x and, from the last wave, the word of w
+  lds_u8* const lds_s = lds + STAGES * STAGE;
+  const unsigned char* xs;
+  {
+    const int64_t m = m0 + wave * 64 + lane;
+    xs = a.x_scale + (m < a.M ? m : a.M - 1) * a.ldxs;
   }
   const unsigned char* ws = a.w_scale + (int64_t)tile_n * a.ldws;
-  const int off = li * 64 + ((g ^ (((li >> 3) & 1) << 1)) << 4);
+  auto stage_scales = [&](int kb) {
+    lds_u8* const to = lds_s + (kb >> 2 & 1) * SCALES;
+    if (wave < XROWS / 64) __builtin_amdgcn_global_load_lds((gvoid_c*)(xs + kb), (__attribute__((address_space(3))) void*)(to + wave * 256), 4, 0, 0);
+    if (wave == 3) __builtin_amdgcn_global_load_lds((gvoid_c*)(ws + kb), (__attribute__((address_space(3))) void*)(to + XROWS * 4), 4, 0, 0);
+  };
+  const int off = li * KS + ((g ^ swizzle(li)) << 4);
   f32x4 acc[NI][MJ];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
@@ -566,64 +577,83 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
     for (int j = 0; j < MJ; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   float sw, sx[MJ];
   auto step = [&](int buf) {
-    const lds_u8* const bw = lds + buf * STAGE + wn * NI * 1024 + off;
-    const lds_u8* const bx = lds + buf * STAGE + (BN + wm * MJ * 16) * 64 + off;
-    bf16x8 fx[MJ][2];
 #pragma unroll
-    for (int j = 0; j < MJ; ++j) {
-      const i32x4 q = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(bx + j * 1024);
-      expand_(q, sx[j], fx[j]);
-    }
+    for (int h = 0; h < KS / 64; ++h) {
+      const lds_u8* const bw = lds + buf * STAGE + wn * NI * 16 * KS + (off ^ (h << 6));
+      const lds_u8* const bx = lds + buf * STAGE + (BN + wm * MJ * 16) * KS + (off ^ (h << 6));
+      bf16x8 fx[MJ][2];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const i32x4 q = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(bw + i * 1024);
-      bf16x8 fw[2];
-      expand_(q, sw, fw);
+      for (int j = 0; j < MJ; ++j) {
+        const i32x4 q = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(bx + j * 16 * KS);
+        expand_(q, sx[j], fx[j]);
+      }
 #pragma unroll
-      for (int j = 0; j < MJ; ++j)
+      for (int i = 0; i < NI; ++i) {
+        const i32x4 q = *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>(bw + i * 16 * KS);
+        bf16x8 fw[2];
+        expand_(q, sw, fw);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[k], fx[j][k], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < MJ; ++j)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[k], fx[j][k], acc[i][j], 0, 0, 0);
+      }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave has read the stage before it reaches the next barrier
   };
-  // Behind wait and barrier the oldest step in flight has landed for every wave, and every wave is done reading the step before it, whose
-  // stage takes the step after next.  Scale bytes are fetched a block ahead and in front of the block's tiles.
+  auto scales = [&](int kb) {
+    const lds_u8* const from = lds_s + (kb >> 2 & 1) * SCALES + (kb & 3);
+    sw = power_(from[XROWS * 4]);
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) sx[j] = power_(from[((wm * MJ + j) * 16 + li) * 4]);
+  };
+  // Behind wait and barrier the oldest step in flight has landed for every wave, and every wave is done reading the step before it, whose stage takes
+  // the next step to be asked for.  (Scale words are not counted: with them in flight a wait waits for more than it has to.)
 #define BLOCKS_ARRIVE(n)                                                                             \
   do {                                                                                               \
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");                                         \
     __builtin_amdgcn_s_barrier();                                                                    \
     __builtin_amdgcn_sched_barrier(0);                                                               \
   } while (0)
-  int wb = ws[0], xb[MJ];
 #pragma unroll
-  for (int j = 0; j < MJ; ++j) xb[j] = xs[j][0];
-  stage(0);
-  stage(1);
-  int cur = 0;
-  for (int kb = 0; kb + 1 < nb; ++kb) {
-    sw = power_(wb);
+  for (int p = 0; p < AHEAD; ++p) {
+    if (p < nb) {
+      if ((p & 3) == 0) stage_scales(p);
 #pragma unroll
-    for (int j = 0; j < MJ; ++j) sx[j] = power_(xb[j]);
-    BLOCKS_ARRIVE(ITS);
-    wb = ws[kb + 1];
-#pragma unroll
-    for (int j = 0; j < MJ; ++j) xb[j] = xs[j][kb + 1];
-    stage(cur >= 1 ? cur - 1 : 2);
-    step(cur);
-    cur = cur == 2 ? 0 : cur + 1;
-    BLOCKS_ARRIVE(ITS);
-    stage(cur >= 1 ? cur - 1 : 2);
-    step(cur);
-    cur = cur == 2 ? 0 : cur + 1;
+      for (int u = 0; u < SUB; ++u) stage(SUB * p + u);
+    }
   }
-  sw = power_(wb);
+  int cur = 0;
+  for (int kb = 0; kb + AHEAD < nb; ++kb) {
 #pragma unroll
-  for (int j = 0; j < MJ; ++j) sx[j] = power_(xb[j]);
-  BLOCKS_ARRIVE(ITS);
-  step(cur);
-  cur = cur == 2 ? 0 : cur + 1;
-  BLOCKS_ARRIVE(0);
-  step(cur);
+    for (int u = 0; u < SUB; ++u) {
+      BLOCKS_ARRIVE(ITS * (STAGES - 2));
+      if (u == 0) {
+        if ((kb + AHEAD & 3) == 0) stage_scales(kb + AHEAD);
+        scales(kb);
+      }
+      stage(cur >= 1 ? cur - 1 : STAGES - 1);
+      step(cur);
+      cur = cur == STAGES - 1 ? 0 : cur + 1;
+    }
+  }
+  auto last = [&](auto left) {                          // `left` blocks are left, all of them in flight
+    constexpr int L = decltype(left)::value;
+    if (L <= nb) {
+      BLOCKS_ARRIVE(ITS * (SUB * L - 1));
+      scales(nb - L);
+      step(cur);
+      cur = cur == STAGES - 1 ? 0 : cur + 1;
+      if constexpr (SUB == 2) {
+        BLOCKS_ARRIVE(ITS * (2 * L - 2));
+        step(cur);
+        cur = cur == STAGES - 1 ? 0 : cur + 1;
+      }
+    }
+  };
+  if constexpr (AHEAD > 2) last(std::integral_constant<int, 3>());
+  if constexpr (AHEAD > 1) last(std::integral_constant<int, 2>());
+  last(std::integral_constant<int, 1>());
+  static_assert((STAGES - 1) % SUB == 0 && AHEAD <= 3, "whole blocks in flight, and scale words of two groups of four");
 #undef BLOCKS_ARRIVE
   if (a.y_type != BLOCKS_F32) __syncthreads();      // every wave is done reading the stages: LDS is the results' now
   const int64_t mw = m0 + wm * MJ * 16;
@@ -649,29 +679,29 @@ void few_(const BlocksDenseArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((dense_few_kernel<T, MT>), dim3((a.N + 15) / 16, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(512), 0, st, a);
 }
 // Tiles of 16 rows per workgroup of the few-rows form, 0 where the tiled form is taken.  The former costs what its workgroups cost -- some 4.2 us up to 256 of
-// them, then in proportion -- and more rows a workgroup read the weights fewer times; the latter takes 14.5 us at k = 2048 for the latency of its steps,
-// but does four times the work in a given time.  So: the fewest rows that need at most 256 workgroups, or as many as there are where those need at
-// most 512.  Measured at k = 2048, us for 1, 2, 4 tiles a workgroup | tiled: 32 x 2048 features 4.2, 5.4, 6.4 | 14.6; 64 x 2048 6.2, 5.5, 7.7 | 14.9; 16 x 8192
-// 6.1, 6.8, 8.2 | 14.3; 32 x 8192 10.3, 8.5, 9.9 | 14.8; 128 x 2048 10.2, 8.6, 7.8 | 15.0; 256 x 2048 18.3, 15.0, 13.2 | 15.0; 512 x 2048 34, 27, 25 | 15.4.
+// them, then in proportion -- and more rows a workgroup read the weights fewer times; the latter takes 11.3 us at k = 2048 for the latency of its steps,
+// but does more work in a given time.  So: the fewest rows that need at most 256 workgroups, or up to 32 rows where those need at most 512.
+// Measured at k = 2048, us for 1, 2, 4 tiles a workgroup | tiled: 64 x 2048 features 6.3, 5.5, 7.7 | 11.4; 16 x 8192 6.1, 6.8, 8.2 | 11.3;
+// 32 x 8192 10.2, 8.5, 9.9 | 11.3; 64 x 8192 18.3, 14.9, 13.2 | 11.7; 128 x 2048 10.3, 8.5, 7.9 | 11.5; 256 x 2048 18.4, 15.0, 13.2 | 11.6.
 int few_tiles_(int64_t M, int N) {
   const int64_t n = (N + 15) / 16;
-  for (int mt = 1;; mt *= 2) {
+  for (int mt = 1; mt <= 4; mt *= 2) {
     const int64_t groups = (M + 16 * mt - 1) / (16 * mt) * n;
-    if (groups <= 256) return mt;
-    if (mt == 4 || M <= 16 * mt) return groups <= 512 ? mt : 0;
+    if (groups <= 256 || (M <= 16 * mt && mt <= 2 && groups <= 512)) return mt;
   }
+  return 0;
 }
 
-template <int BM, int WN>
+template <int BM, int WN, int STAGES, int KS>
 void tile_(const BlocksDenseArgs& a, hipStream_t st) {
-  const int lds = max(3 * (128 + BM) * 64, min(a.lds_floor, 128 * 1024));
+  const int lds = max(STAGES * (128 + BM) * KS + 2 * (max(BM, 64) + 64) * 4, min(a.lds_floor, 128 * 1024));
   const int64_t tiles = (int64_t)((a.N + 127) / 128) * ((a.M + BM - 1) / BM), grid = (tiles + 7) / 8 * 8;
   if (grid * 256 > 0xffffffffLL) throw std::runtime_error("launch_blocks_dense: too many rows for one launch");
   static std::once_flag once[16];
   int dev = 0;
   (void)hipGetDevice(&dev);
-  std::call_once(once[dev & 15], []() { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(dense_tile_kernel<BM, WN>), hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024); });
-  hipLaunchKernelGGL((dense_tile_kernel<BM, WN>), dim3((unsigned)grid), dim3(256), lds, st, a);
+  std::call_once(once[dev & 15], []() { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(dense_tile_kernel<BM, WN, STAGES, KS>), hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024); });
+  hipLaunchKernelGGL((dense_tile_kernel<BM, WN, STAGES, KS>), dim3((unsigned)grid), dim3(256), lds, st, a);
 }
 
 }  // namespace
@@ -768,12 +798,14 @@ void launch_blocks_dense(const BlocksDenseArgs& args, void* workspace, hipStream
     }
     return;
   }
-  // Rows of a tile: larger tiles do more work for what they stage, smaller ones fill the chip sooner.  Measured at k = 2048, us for 64 / 128 / 256 rows:
-  // 512 x 8192 features 24.6 / 27.8 / 37.0 and 2048 x 2048 24.0 / 26.8 / 36.9 (256 tiles of 128 rows); 1024 x 8192 43.0 / 40.1 / 40.0 and 6144 x 2048
-  // in blocks 59.7 / 51.9 / 55.5 (256 and 384 tiles of 256 rows: less than two workgroups for every compute unit); 2048 x 8192 82.2 / 74.0 / 65.5;
-  // 6144 x 8192 f16 221 / 193 / 173; 32000 x 8192 1253 / 1068 / 981.
+  // Rows of a tile: larger tiles do more work for what they stage, smaller ones fill the chip sooner.  Measured at k = 2048, us for 32 / 64 / 128 / 256 rows:
+  // 512 x 2048 features 12.2 / 14.7 / 23.2 / 33.7 and 1024 x 2048 15.8 / 15.8 / 23.8 / 34.2 (256 and 512 tiles of 32 rows); 512 x 8192 29.1 / 23.1 / 26.3 /
+  // 35.9 and 2048 x 2048 27.2 / 21.8 / 25.1 / 35.7 (256 tiles of 128 rows); 1024 x 8192 51.5 / 40.9 / 37.8 / 38.3 and 6144 x 2048 in blocks
+  // 74.7 / 55.3 / 49.5 / 55.8 (256 and 384 tiles of 256 rows: less than two workgroups for every compute unit); 2048 x 8192 98 / 77 / 69 / 63;
+  // 6144 x 8192 f16 280 / 217 / 179 / 162.
   const int64_t tiles_n = (a.N + 127) / 128;
-  if (tiles_n * ((a.M + 127) / 128) <= 256) tile_<64, 2>(a, st);
-  else if (tiles_n * ((a.M + 255) / 256) < 512) tile_<128, 1>(a, st);
-  else tile_<256, 1>(a, st);
+  if (tiles_n * ((a.M + 31) / 32) <= 256) tile_<32, 4, 3, 128>(a, st);
+  else if (tiles_n * ((a.M + 127) / 128) <= 256) tile_<64, 2, 3, 128>(a, st);
+  else if (tiles_n * ((a.M + 255) / 256) < 512) tile_<128, 1, 3, 64>(a, st);
+  else tile_<256, 1, 3, 64>(a, st);
 }

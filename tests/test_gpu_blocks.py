@@ -418,3 +418,16 @@ def test_parts_of_block_tensors(m):
     np.testing.assert_array_equal(host(blocks.dense_blocks(x1, w1, dtype=torch.float32)), R.dense(xd[4:4 + m, :256], wd[128:, :256]))
     p = torch.ones(4, 300, device="cuda", requires_grad=True)
     assert not blocks.dense_blocks(p, w, dtype=torch.float32).requires_grad and not blocks.dequantize_blocks(blocks.quantize_blocks(p)).requires_grad
+
+
+@pytest.mark.parametrize("k", [1, 128, 200, 300, 500, 640, 1025])
+@pytest.mark.parametrize("m,n", [(300, 900), (999, 1100), (2500, 2100)])
+def test_dense_blocks_along_k(m, n, k):
+    """Tiles of 32, 64 and 128 rows over one block along k, fewer than they keep in flight, and more than one word of scale bytes; equal in every bit."""
+    rng = np.random.default_rng(m + k)
+    x, xd = whole_blocks(rng, m, k, 1)
+    w, wd = whole_blocks(rng, n, k, 128)
+    want = R.dense(xd, wd, None, None)
+    for t, dt in TYPES.items():
+        np.testing.assert_array_equal(host(blocks.dense_blocks(x, w, dtype=dt)), host(torch.from_numpy(want).float().to(dt)), err_msg=t)
+    check_blocks(blocks.dense_blocks(x, w, dtype=E4M3), want, 1)
