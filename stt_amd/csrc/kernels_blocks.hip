@@ -535,7 +535,7 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
   }
   const int n0 = tile_n * BN;
   const int64_t m0 = tile_m * BM;
-  if (tid < BN) s_bias[tid] = a.bias && n0 + tid < a.N ? a.bias[n0 + tid] : 0.0f;      // (visible behind the first barrier below)
+  if (tid < BN) s_bias[tid] = a.bias && n0 + tid < a.N ? a.bias[n0 + tid] : 0.0f;      // (visible behind the first barrier below, which the wait for this write stands in front of)
   const int nb = (a.K + 127) >> 7;
   auto swizzle = [](int r) { return KS == 64 ? ((r >> 3) & 1) << 1 : (r >> 1) & 7; };
   const unsigned char* src[ITS];
@@ -622,6 +622,8 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
       for (int u = 0; u < SUB; ++u) stage(SUB * p + u);
     }
   }
+  // The barriers below wait for no LDS write by themselves, and one block along k in a step of 128 passes a single one before f32 results read the biases.
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   int cur = 0;
   for (int kb = 0; kb + AHEAD < nb; ++kb) {
 #pragma unroll

@@ -431,3 +431,20 @@ def test_dense_blocks_along_k(m, n, k):
     for t, dt in TYPES.items():
         np.testing.assert_array_equal(host(blocks.dense_blocks(x, w, dtype=dt)), host(torch.from_numpy(want).float().to(dt)), err_msg=t)
     check_blocks(blocks.dense_blocks(x, w, dtype=E4M3), want, 1)
+
+
+@pytest.mark.parametrize("k", [1, 100, 128, 129])
+@pytest.mark.parametrize("m,n", [(300, 900), (999, 1100), (2500, 2100)])
+def test_dense_bias_over_one_block(m, n, k):
+    """The biases are in LDS before any wave adds them, also where a tile passes one barrier only: one block along k (and two, at 129), a bias, tiles of 32, 64
+    and 128 rows, every type of result; equal in every bit."""
+    rng = np.random.default_rng(m + k)
+    x, xd = whole_blocks(rng, m, k, 1)
+    w, wd = whole_blocks(rng, n, k, 128)
+    bias = rng.integers(-900, 901, n) / 4.0
+    bg = torch.from_numpy(bias).float().cuda()
+    for clip in (None, 100.0):
+        want = R.dense(xd, wd, bias, clip)
+        for t, dt in TYPES.items():
+            np.testing.assert_array_equal(host(blocks.dense_blocks(x, w, bg, relu_clip=clip, dtype=dt)), host(torch.from_numpy(want).float().to(dt)), err_msg="%s %s" % (t, clip))
+        check_blocks(blocks.dense_blocks(x, w, bg, relu_clip=clip, dtype=E4M3), want, 1)
