@@ -179,7 +179,9 @@ STTX_EXPORT int STTX_GetGeometry(const ModelState* aCtx, int* aOut10);
  * input may be anything from 0 (every row the same one); an output's is at least its columns.  Zero rows are a call that does nothing.  Outputs
  * must not overlap inputs or each other.  The calls enqueue on aStream (a hipStream_t of any device; NULL = the current device's null stream),
  * allocate nothing, keep nothing and do not wait: they may be captured into a HIP graph, and called from several threads at once.
- * STT_ERR_INVALID_SHAPE (a line on stderr says what): an argument is outside the above, nothing was enqueued. */
+ * STT_ERR_INVALID_SHAPE (a line on stderr says what): an argument is outside the above, or there are more rows than a launch can hold (rows times
+ * columns / 512 above 2^38 - 2^22 for rows of 1 x 128 blocks, more than 2^24 - 8 tiles of 128 features by 256 rows for a dense layer: beyond a GPU's memory
+ * either way); nothing was enqueued. */
 enum STTX_ElementType { STTX_F32 = 0, STTX_F16 = 1, STTX_BF16 = 2, STTX_E4M3 = 3 };
 /* aX [aRows][aCols] of aType (STTX_F32, STTX_F16, STTX_BF16) -> aQ, aScale in blocks of aBlockRows (1 or 128) x 128.  With 1-row blocks up to
  * 2^31 - 1 rows, with 128-row blocks up to 128 * 65535. */

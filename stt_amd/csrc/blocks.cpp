@@ -76,7 +76,7 @@ int STTX_QuantizeBlocks(const void* aX, int aType, long long aRows, long long aC
   return entry("STTX_QuantizeBlocks", [&]() {
     want_sizes(aRows, aCols);
     want(aBlockRows == 1 || aBlockRows == 128, "blocks have 1 or 128 rows");
-    want(aBlockRows == 1 || aRows <= 128LL * 65535, "rows out of range");
+    want(aBlockRows == 1 ? blocks_rows_fit(aRows, (int)aCols) : blocks_tiles_fit(aRows), "too many rows for one launch");
     want_plain(aX, aType, aRows, aCols, aLdX, false);
     want_blocks(aQ, aLdQ, aScale, aLdScale, aRows, aCols);
     if (aRows == 0) return;
@@ -95,6 +95,7 @@ int STTX_DequantizeBlocks(const unsigned char* aQ, long long aLdQ, const unsigne
   return entry("STTX_DequantizeBlocks", [&]() {
     want_sizes(aRows, aCols);
     want(aBlockRows == 1 || aBlockRows == 128, "blocks have 1 or 128 rows");
+    want(blocks_rows_fit(aRows, (int)aCols), "too many rows for one launch");
     want_blocks(aQ, aLdQ, aScale, aLdScale, aRows, aCols);
     want_plain(aY, aType, aRows, aCols, aLdY, true);
     if (aRows == 0) return;
@@ -126,6 +127,7 @@ int STTX_DenseBlocks(const STTX_DenseBlocksArgs* aArgs) {
     want(aligned(c.bias, 4), "pointer not aligned to its element type");
     if (c.y_type == STTX_E4M3) want_blocks(c.y, c.y_ld, c.y_scale, c.y_scale_ld, c.rows, c.out);
     else want_plain(c.y, c.y_type, c.rows, c.out, c.y_ld, true);
+    want(blocks_dense_fits(c.x_type, c.y_type, c.rows, (int)c.out, (int)c.in), "too many rows for one launch");
     want(c.relu_clip > 0.0f || c.relu_clip == 0.0f, "the clip of the ReLU is positive, or 0 for no ReLU");
     if (c.rows == 0) return;
     const unsigned long long need = STTX_DenseBlocksWorkspace(c.x_type, c.y_type, c.rows, c.in, c.out);

@@ -166,6 +166,10 @@ struct BlocksDenseArgs {
   int ordered;              // 1: every sum runs along k in ONE order however many rows there are (the tiled form always): a row's results do not depend on the rows beside it
   int lds_floor;            // as DenseArgs::lds_floor
 };
+// Whether a grid holds so many rows: the launches below take it for granted.  Rows of 1 x 128 blocks there and back; of 128 x 128 blocks; a dense layer.
+bool blocks_rows_fit(int64_t rows, int cols);
+bool blocks_tiles_fit(int64_t rows);
+bool blocks_dense_fits(int x_type, int y_type, int64_t M, int N, int K, int ordered = 0);
 void launch_blocks_quantize(const BlocksQuantArgs& a, hipStream_t st);
 void launch_blocks_dequantize(const BlocksDequantArgs& a, hipStream_t st);
 size_t blocks_dense_workspace(int x_type, int y_type, int64_t M, int N, int K, int ordered = 0);   // bytes, at a multiple of 16

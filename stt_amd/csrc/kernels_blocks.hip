@@ -19,7 +19,6 @@
 #include <stdint.h>
 
 #include <mutex>
-#include <stdexcept>
 #include <type_traits>
 
 #include "kernels.h"
@@ -669,11 +668,12 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
   }
 }
 
-// Workgroups of four waves, one item each; over two dimensions, because a dimension holds less than 2^32 threads.
-dim3 rows_grid_(int64_t items) {
-  const int64_t blocks = (items + 3) / 4, x = blocks < (1 << 20) ? blocks : 1 << 20, y = (blocks + x - 1) / x;
-  if (y > 65535) throw std::runtime_error("block operators: too many rows for one launch");
-  return dim3((unsigned)x, (unsigned)y);
+// Workgroups of four waves, one item (four blocks of a row) each; over two dimensions, because a dimension holds less than 2^32 threads.
+constexpr int64_t kGridX = 1 << 20, kGridY = 65535;
+int64_t row_groups_(int64_t rows, int cols) { return (rows * (((int64_t)cols + 511) / 512) + 3) / 4; }
+dim3 rows_grid_(int64_t rows, int cols) {
+  const int64_t blocks = row_groups_(rows, cols), x = blocks < kGridX ? blocks : kGridX;
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
 }
 
 template <int T, int MT>
@@ -694,11 +694,24 @@ int few_tiles_(int64_t M, int N) {
   return 0;
 }
 
+// Rows of a tile: larger tiles do more work for what they stage, smaller ones fill the chip sooner.  Measured at k = 2048, us for 32 / 64 / 128 / 256 rows:
+// 512 x 2048 features 12.2 / 14.7 / 23.2 / 33.7 and 1024 x 2048 15.8 / 15.8 / 23.8 / 34.2 (256 and 512 tiles of 32 rows); 512 x 8192 29.1 / 23.1 / 26.3 /
+// 35.9 and 2048 x 2048 27.2 / 21.8 / 25.1 / 35.7 (256 tiles of 128 rows); 1024 x 8192 51.5 / 40.9 / 37.8 / 38.3 and 6144 x 2048 in blocks
+// 74.7 / 55.3 / 49.5 / 55.8 (256 and 384 tiles of 256 rows: less than two workgroups for every compute unit); 2048 x 8192 98 / 77 / 69 / 63;
+// 6144 x 8192 f16 280 / 217 / 179 / 162.
+int tile_rows_(int64_t M, int N) {
+  const int64_t tiles_n = ((int64_t)N + 127) / 128;
+  if (tiles_n * ((M + 31) / 32) <= 256) return 32;
+  if (tiles_n * ((M + 127) / 128) <= 256) return 64;
+  return tiles_n * ((M + 255) / 256) < 512 ? 128 : 256;
+}
+// Workgroups of the tiled form: a multiple of eight, one run of tiles for every XCD.
+int64_t tile_groups_(int64_t M, int N, int rows) { return (((int64_t)N + 127) / 128 * ((M + rows - 1) / rows) + 7) / 8 * 8; }
+
 template <int BM, int WN, int STAGES, int KS>
 void tile_(const BlocksDenseArgs& a, hipStream_t st) {
   const int lds = max(STAGES * (128 + BM) * KS + 2 * (max(BM, 64) + 64) * 4, min(a.lds_floor, 128 * 1024));
-  const int64_t tiles = (int64_t)((a.N + 127) / 128) * ((a.M + BM - 1) / BM), grid = (tiles + 7) / 8 * 8;
-  if (grid * 256 > 0xffffffffLL) throw std::runtime_error("launch_blocks_dense: too many rows for one launch");
+  const int64_t grid = tile_groups_(a.M, a.N, BM);
   static std::once_flag once[16];
   int dev = 0;
   (void)hipGetDevice(&dev);
@@ -708,20 +721,20 @@ void tile_(const BlocksDenseArgs& a, hipStream_t st) {
 
 }  // namespace
 
+bool blocks_rows_fit(int64_t rows, int cols) { return row_groups_(rows, cols) <= kGridX * kGridY; }
+bool blocks_tiles_fit(int64_t rows) { return (rows + 127) / 128 <= kGridY; }
+
 void launch_blocks_quantize(const BlocksQuantArgs& a, hipStream_t st) {
   if (a.rows < 1) return;
-  const int64_t quads = (a.cols + 511) / 512;
   if (a.block_rows == 1) {
-    const dim3 grid = rows_grid_(a.rows * quads), block(256);
+    const dim3 grid = rows_grid_(a.rows, a.cols), block(256);
     switch (a.type) {
       case BLOCKS_F32: hipLaunchKernelGGL(quantize_rows_kernel<BLOCKS_F32>, grid, block, 0, st, a); break;
       case BLOCKS_F16: hipLaunchKernelGGL(quantize_rows_kernel<BLOCKS_F16>, grid, block, 0, st, a); break;
       default: hipLaunchKernelGGL(quantize_rows_kernel<BLOCKS_BF16>, grid, block, 0, st, a); break;
     }
   } else {
-    const int64_t tiles = (a.rows + 127) / 128;
-    if (tiles > 65535) throw std::runtime_error("launch_blocks_quantize: too many rows for one launch");
-    const dim3 grid((unsigned)quads * 4, (unsigned)tiles), block(256);
+    const dim3 grid((unsigned)(a.cols + 511) / 512 * 4, (unsigned)((a.rows + 127) / 128)), block(256);
     switch (a.type) {
       case BLOCKS_F32: hipLaunchKernelGGL(quantize_tiles_kernel<BLOCKS_F32>, grid, block, 0, st, a); break;
       case BLOCKS_F16: hipLaunchKernelGGL(quantize_tiles_kernel<BLOCKS_F16>, grid, block, 0, st, a); break;
@@ -732,7 +745,7 @@ void launch_blocks_quantize(const BlocksQuantArgs& a, hipStream_t st) {
 
 void launch_blocks_dequantize(const BlocksDequantArgs& a, hipStream_t st) {
   if (a.rows < 1) return;
-  const dim3 grid = rows_grid_(a.rows * ((a.cols + 511) / 512)), block(256);
+  const dim3 grid = rows_grid_(a.rows, a.cols), block(256);
   switch (a.type) {
     case BLOCKS_F32: hipLaunchKernelGGL(dequantize_kernel<BLOCKS_F32>, grid, block, 0, st, a); break;
     case BLOCKS_F16: hipLaunchKernelGGL(dequantize_kernel<BLOCKS_F16>, grid, block, 0, st, a); break;
@@ -773,6 +786,14 @@ size_t blocks_dense_workspace(int x_type, int y_type, int64_t M, int N, int K, i
   return p.x_bytes + p.y_bytes;
 }
 
+bool blocks_dense_fits(int x_type, int y_type, int64_t M, int N, int K, int ordered) {
+  if (M < 1) return true;
+  const Plan p(x_type, y_type, M, N, K, ordered);
+  if (p.x_bytes && !blocks_rows_fit(M, K)) return false;
+  if (p.mt) return !p.y_bytes || blocks_rows_fit(M, N);
+  return tile_groups_(M, N, tile_rows_(M, N)) * 256 <= 0xffffffffLL;
+}
+
 void launch_blocks_dense(const BlocksDenseArgs& args, void* workspace, hipStream_t st) {
   BlocksDenseArgs a = args;
   if (a.M < 1) return;
@@ -800,14 +821,10 @@ void launch_blocks_dense(const BlocksDenseArgs& args, void* workspace, hipStream
     }
     return;
   }
-  // Rows of a tile: larger tiles do more work for what they stage, smaller ones fill the chip sooner.  Measured at k = 2048, us for 32 / 64 / 128 / 256 rows:
-  // 512 x 2048 features 12.2 / 14.7 / 23.2 / 33.7 and 1024 x 2048 15.8 / 15.8 / 23.8 / 34.2 (256 and 512 tiles of 32 rows); 512 x 8192 29.1 / 23.1 / 26.3 /
-  // 35.9 and 2048 x 2048 27.2 / 21.8 / 25.1 / 35.7 (256 tiles of 128 rows); 1024 x 8192 51.5 / 40.9 / 37.8 / 38.3 and 6144 x 2048 in blocks
-  // 74.7 / 55.3 / 49.5 / 55.8 (256 and 384 tiles of 256 rows: less than two workgroups for every compute unit); 2048 x 8192 98 / 77 / 69 / 63;
-  // 6144 x 8192 f16 280 / 217 / 179 / 162.
-  const int64_t tiles_n = (a.N + 127) / 128;
-  if (tiles_n * ((a.M + 31) / 32) <= 256) tile_<32, 4, 3, 128>(a, st);
-  else if (tiles_n * ((a.M + 127) / 128) <= 256) tile_<64, 2, 3, 128>(a, st);
-  else if (tiles_n * ((a.M + 255) / 256) < 512) tile_<128, 1, 3, 64>(a, st);
-  else tile_<256, 1, 3, 64>(a, st);
+  switch (tile_rows_(a.M, a.N)) {
+    case 32: tile_<32, 4, 3, 128>(a, st); break;
+    case 64: tile_<64, 2, 3, 128>(a, st); break;
+    case 128: tile_<128, 1, 3, 64>(a, st); break;
+    default: tile_<256, 1, 3, 64>(a, st); break;
+  }
 }

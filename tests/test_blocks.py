@@ -120,3 +120,17 @@ def test_python_refuses():
         with pytest.raises(ValueError):
             blocks.dequantize_blocks(blocks.BlockTensor(v, s, cols, br))
     assert repr(w) == "BlockTensor(300 x 200, blocks of 128 x 128)" and w.shape == (300, 200)
+
+
+def test_more_rows_than_a_launch_holds(L, capfd):
+    """Refused with the other arguments, before anything is enqueued: 2^39 groups of four blocks there and back; 2^24 tiles of 256 x 128 of a dense layer, with x
+    in blocks and with an x that a quantising launch would go in front of."""
+    many, wide = (1 << 31) - 1, 1 << 17
+    assert _quant(L, rows=many, cols=wide, ldx=0, ldq=wide, lds=wide // 128) == INVALID_SHAPE
+    assert "too many rows" in capfd.readouterr().err
+    assert _dequant(L, rows=many, cols=wide, ldq=wide, lds=wide // 128, ldy=wide) == INVALID_SHAPE
+    assert "too many rows" in capfd.readouterr().err
+    assert _dense(L, rows=many, out=129, y_ld=129) == INVALID_SHAPE
+    assert "too many rows" in capfd.readouterr().err
+    assert _dense(L, rows=many, out=129, y_ld=129, x_type=1, x_ld=0, workspace=0x80000, workspace_bytes=1 << 60) == INVALID_SHAPE
+    assert "too many rows" in capfd.readouterr().err
