@@ -175,9 +175,9 @@ STTX_EXPORT int STTX_GetGeometry(const ModelState* aCtx, int* aOut10);
  * becomes the e4m3 nearest to x / 2^e, ties to even; infinities and NaN become NaN and do not move their block's power.  Reading back rounds
  * once, to the type asked for.
  *
- * All pointers are device pointers; rows have unit column stride, row strides are in elements (bytes for values and scales).  A row stride of an
- * input may be anything from 0 (every row the same one); an output's is at least its columns.  Zero rows are a call that does nothing.  Outputs
- * must not overlap inputs or each other.  The calls enqueue on aStream (a hipStream_t of any device; NULL = the current device's null stream),
+ * All pointers are device pointers; rows have unit column stride, row strides are in elements (bytes for values and scales).  The row stride of an
+ * f32 / f16 / bf16 input may be anything from 0 (every row the same one), an output's is at least its columns; those of a matrix in blocks, input or
+ * output, one row or many, are at least its padded columns and blocks.  Zero rows are a call that does nothing.  Outputs must not overlap inputs or each other.  The calls enqueue on aStream (a hipStream_t of any device; NULL = the current device's null stream),
  * allocate nothing, keep nothing and do not wait: they may be captured into a HIP graph, and called from several threads at once.
  * STT_ERR_INVALID_SHAPE (a line on stderr says what): an argument is outside the above, or there are more rows than a launch can hold (rows times
  * columns / 512 above 2^38 - 2^22 for rows of 1 x 128 blocks, more than 2^24 - 8 tiles of 128 features by 256 rows for a dense layer: beyond a GPU's memory

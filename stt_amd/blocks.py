@@ -39,7 +39,8 @@ def _entry():
 
 class BlockTensor(object):
     """A matrix in blocks: `values` float8_e4m3fn [rows][cols rounded up to 128], `scale` uint8 [rows or row blocks][blocks rounded up to 4] (byte s
-    stands for 2^(s - 127)), `cols` columns that count, blocks of `block_rows` (1 or 128) x 128.  The padding of `values` is zeros."""
+    stands for 2^(s - 127)), `cols` columns that count, blocks of `block_rows` (1 or 128) x 128.  The padding of `values` is zeros.  Parts of larger
+    matrices will do whose rows do not overlap and start at multiples of 16 (values) and 4 bytes (scale)."""
     __slots__ = ("values", "scale", "cols", "block_rows")
 
     def __init__(self, values, scale, cols, block_rows=1):
@@ -83,17 +84,25 @@ def _bad_blocks(b, what, block_rows):
         return ValueError("%s: scales %s do not cover the blocks of %d x %d values" % (what, tuple(s.shape), v.shape[0], b.cols))
     if not v.is_cuda or v.device != s.device:
         return ValueError("%s: values and scales have to be in one GPU's memory, got %s and %s" % (what, v.device, s.device))
-    return ValueError("%s: columns have to be contiguous (stride 1)" % what)
+    if v.stride(1) != 1 or s.stride(1) != 1:
+        return ValueError("%s: columns have to be contiguous (stride 1)" % what)
+    return ValueError("%s: rows must not overlap and have to start at multiples of 16 bytes (values) and 4 bytes (scale), got strides of %d and %d from 0x%x and 0x%x" %
+                      (what, v.stride(0), s.stride(0), v.data_ptr(), s.data_ptr()))
 
 
 def _blocks(b, what, block_rows):
-    """(rows, cols, row stride of the values, of the scales, device index); block_rows: the ones that may be"""
+    """(rows, cols, values' address and row stride, scales' address and row stride, device index); block_rows: the ones that may be.  The stride of a single row,
+    which torch leaves open, is the width."""
     v, s, cols, br = b.values, b.scale, b.cols, b.block_rows
     vs, ss = v.shape, s.shape
     if (v.dtype is not E4M3 or s.dtype is not _UINT8 or len(vs) != 2 or len(ss) != 2 or br not in block_rows or cols < 1 or vs[1] < -(-cols // BLOCK) * BLOCK or
             ss[0] * br < vs[0] or ss[1] < -(-cols // 512) * 4 or not v.is_cuda or v.get_device() != s.get_device() or v.stride(1) != 1 or s.stride(1) != 1):
         raise _bad_blocks(b, what, block_rows)
-    return vs[0], cols, v.stride(0), s.stride(0), v.get_device()
+    wide, words = -(-cols // BLOCK) * BLOCK, -(-cols // 512) * 4
+    ldq, lds, q, scale = v.stride(0) if vs[0] > 1 else wide, s.stride(0) if ss[0] > 1 else words, v.data_ptr(), s.data_ptr()
+    if ldq < wide or lds < words or (ldq | q) & 15 or (lds | scale) & 3:
+        raise _bad_blocks(b, what, block_rows)
+    return vs[0], cols, q, ldq, scale, lds, v.get_device()
 
 
 def _call(index, fn, *args):
@@ -121,12 +130,12 @@ def quantize_blocks(x, block_rows=1):
 
 def dequantize_blocks(b, dtype=torch.float32):
     """BlockTensor -> [rows][cols] of `dtype` (float32, float16, bfloat16), one rounding."""
-    rows, cols, ldq, lds, index = _blocks(b, "b", (1, BLOCK))
+    rows, cols, q, ldq, scale, lds, index = _blocks(b, "b", (1, BLOCK))
     kind = _PLAIN.get(dtype, -1)
     if kind < 0:
         raise ValueError("dtype: float32, float16 or bfloat16 is wanted, got %s" % (dtype,))
     y = b.scale.new_empty((rows, cols), dtype=dtype)
-    _call(index, (_lib or _entry()).STTX_DequantizeBlocks, b.values.data_ptr(), ldq, b.scale.data_ptr(), lds, rows, cols, b.block_rows, y.data_ptr(), kind, cols, _raw_stream(index))
+    _call(index, (_lib or _entry()).STTX_DequantizeBlocks, q, ldq, scale, lds, rows, cols, b.block_rows, y.data_ptr(), kind, cols, _raw_stream(index))
     return y
 
 
@@ -135,10 +144,10 @@ def dense_blocks(x, w, bias=None, relu_clip=None, dtype=torch.float16):
 
     x: [rows][in] float32 / float16 / bfloat16 (quantised within the call) or a BlockTensor in blocks of 1 x 128; w: BlockTensor [out][in] in blocks of
     128 x 128; bias: float32 [out].  Returns [rows][out] of `dtype`, or for dtype float8_e4m3fn a BlockTensor in blocks of 1 x 128."""
-    out, inner, w_ld, w_scale_ld, index = _blocks(w, "w", (BLOCK,))
+    out, inner, w_ptr, w_ld, w_scale, w_scale_ld, index = _blocks(w, "w", (BLOCK,))
     if isinstance(x, BlockTensor):
-        rows, cols, x_ld, x_scale_ld, at = _blocks(x, "x", (1,))
-        kind, x_ptr, x_scale = _E4M3, x.values.data_ptr(), x.scale.data_ptr()
+        rows, cols, x_ptr, x_ld, x_scale, x_scale_ld, at = _blocks(x, "x", (1,))
+        kind = _E4M3
     else:
         kind, rows, cols, x_ld, at = _plain(x, "x")
         x_ptr, x_scale, x_scale_ld = x.data_ptr(), 0, 0
@@ -169,7 +178,7 @@ def dense_blocks(x, w, bias=None, relu_clip=None, dtype=torch.float16):
         y_ptr, y_ld, y_scale, y_scale_ld = y.data_ptr(), out, 0, 0
     need = L.STTX_DenseBlocksWorkspace(kind, y_kind, rows, inner, out) if kind != _E4M3 or y_kind == _E4M3 else 0
     work = w.scale.new_empty(need) if need else None         # torch's allocator: this stream's, or the capturing graph's own
-    args = _ARGS(x_ptr, x_scale, w.values.data_ptr(), w.scale.data_ptr(), b_ptr, y_ptr, y_scale, work.data_ptr() if need else 0, _raw_stream(index),
+    args = _ARGS(x_ptr, x_scale, w_ptr, w_scale, b_ptr, y_ptr, y_scale, work.data_ptr() if need else 0, _raw_stream(index),
                                   x_ld, x_scale_ld, w_ld, w_scale_ld, y_ld, y_scale_ld, need, rows, inner, out, kind, y_kind, clip)
     _call(index, L.STTX_DenseBlocks, args)
     return y

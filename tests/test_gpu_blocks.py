@@ -448,3 +448,38 @@ def test_dense_bias_over_one_block(m, n, k):
         for t, dt in TYPES.items():
             np.testing.assert_array_equal(host(blocks.dense_blocks(x, w, bg, relu_clip=clip, dtype=dt)), host(torch.from_numpy(want).float().to(dt)), err_msg="%s %s" % (t, clip))
         check_blocks(blocks.dense_blocks(x, w, bg, relu_clip=clip, dtype=E4M3), want, 1)
+
+
+def test_block_tensors_of_one_row():
+    """The stride of a single row means nothing: any will do, of values, of scales and of a plain x."""
+    rng = np.random.default_rng(21)
+    xb, xd = whole_blocks(rng, 1, 300, 1)
+    wb, wd = whole_blocks(rng, 100, 300, 128)
+    w1, w1d = whole_blocks(rng, 1, 300, 128)
+    for ld, lds in ((1, 1), (0, 0), (7, 3), (385, 5)):
+        x = blocks.BlockTensor(xb.values.as_strided((1, 384), (ld, 1)), xb.scale.as_strided((1, 4), (lds, 1)), 300)
+        w = blocks.BlockTensor(wb.values, wb.scale.as_strided((1, 4), (lds, 1)), 300, 128)
+        np.testing.assert_array_equal(host(blocks.dequantize_blocks(x)), xd)
+        np.testing.assert_array_equal(host(blocks.dense_blocks(x, w, dtype=torch.float32)), R.dense(xd, wd))
+        one = blocks.BlockTensor(w1.values.as_strided((1, 384), (ld, 1)), w1.scale.as_strided((1, 4), (lds, 1)), 300, 128)
+        np.testing.assert_array_equal(host(blocks.dense_blocks(x, one, dtype=torch.float32)), R.dense(xd, w1d))
+        np.testing.assert_array_equal(host(blocks.dense_blocks(torch.from_numpy(xd).half().cuda().as_strided((1, 300), (ld, 1)), w, dtype=torch.float32)), R.dense(xd, wd))
+
+
+def test_block_tensors_whose_rows_are_refused():
+    """Rows that overlap or start elsewhere than at 16 bytes (values) or 4 bytes (scales) are told as such, before the entry is called."""
+    rng = np.random.default_rng(22)
+    x, _ = whole_blocks(rng, 6, 600, 1)
+    w, _ = whole_blocks(rng, 300, 600, 128)
+    flat, marks = x.values.view(torch.uint8).reshape(-1), x.scale.reshape(-1)
+    for v, s, cols in ((x.values[:1].expand(6, 640), x.scale, 600), (x.values, x.scale[:1].expand(6, 8), 600),
+                       (flat.as_strided((4, 640), (512, 1)).view(E4M3), x.scale, 600), (flat.as_strided((4, 640), (648, 1)).view(E4M3), x.scale, 600),
+                       (flat.as_strided((4, 640), (640, 1), 8).view(E4M3), x.scale, 600), (x.values, marks.as_strided((6, 8), (6, 1)), 600),
+                       (x.values[:4], marks.as_strided((4, 8), (9, 1)), 600), (x.values[:, 128:], x.scale[:, 1:], 100), (x.values[:1], x.scale[:1, 2:], 100)):
+        b = blocks.BlockTensor(v, s, cols)
+        part = blocks.BlockTensor(w.values, w.scale, cols, 128)
+        for call in (lambda: blocks.dequantize_blocks(b), lambda: blocks.dense_blocks(b, part)):
+            with pytest.raises(ValueError, match="multiples of 16"):
+                call()
+    with pytest.raises(ValueError, match="multiples of 16"):
+        blocks.dense_blocks(x, blocks.BlockTensor(w.values, w.scale[:1].expand(3, 8), 600, 128))
