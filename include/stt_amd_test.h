@@ -37,6 +37,8 @@ STTX_EXPORT int STTX_TestDense(int aM, int aN, int aK, const float* aX, const fl
 STTX_EXPORT int STTX_TestDenseHybrid(const float* aX, unsigned int aM, unsigned int aK, const signed char* aWq, const float* aWScale, unsigned int aNScales,
                                       const float* aBias, unsigned int aN, float* aY, signed char* aQ, float* aRowScale, unsigned int aReps, float* aElapsedMs,
                                       int aEpi, float aClip);
+/* Host only: the hardware queues the engine takes this process to have when it places its streams (GPU_MAX_HW_QUEUES, four where that is not set). */
+STTX_EXPORT int STTX_TestHwQueues(void);
 /* Test hook (int8 path): rows that took the recurrent step's slow path (max |h| above max |x_t|: both halves again at the joint scale) since the
  * model was created, over every engine form; waits for everything in flight.  0 rows on a float model. */
 STTX_EXPORT int STTX_DebugSlowRows(ModelState* aCtx, unsigned int* aRows);

@@ -1453,6 +1453,7 @@ int STTX_TestDense(int M, int N, int K, const float* aX, const float* aW, const 
 // scales); aReps timed repetitions of quantisation + product (HIP events) -> *aElapsedMs per repetition.
 int STTX_GetAcousticMode(const ModelState* m) { return m ? m->arithmetic() : 0; }
 #ifdef STT_TEST_HOOKS
+int STTX_TestHwQueues(void) { return hw_queues(); }
 int STTX_DebugSlowRows(ModelState* m, unsigned int* aRows) {
   return guarded([&]() {
     if (!m || !aRows) return (int)STT_ERR_INVALID_SHAPE;

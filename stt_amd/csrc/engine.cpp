@@ -371,10 +371,9 @@ void ModelState::place_batch_streams(hipStream_t* slot_streams, int n_slots, boo
   for (int i = 0; i < n_slots; ++i) {
     hipStream_t st = nullptr;
     if (spread_searches) {
-      // A process of four hardware queues (GPU_MAX_HW_QUEUES): a class is ONE queue, whose work runs in order -- searches stay off the GEMM engine's
+      // A process of four hardware queues (the runtime's default): a class is ONE queue, whose work runs in order -- searches stay off the GEMM engine's
       // and the recurrence's (code-point scorer, beam 1024: 28.5 ms per batch, 41.4 with a search in front of each; unplaced 28.1).
-      const char* queues = getenv("GPU_MAX_HW_QUEUES");
-      const bool one_queue = queues && atoi(queues) > 0 && atoi(queues) <= 4;
+      const bool one_queue = hw_queues() <= 4;
       const int order[4] = {ks, ko, one_queue ? ks : kr, one_queue ? ko : 0};
       for (int k = 0; k < 4 && !st; ++k) st = take(order[(i + k) & 3]);
     } else {

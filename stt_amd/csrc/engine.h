@@ -68,6 +68,7 @@ struct PinnedBuf {
 // A stream of the engine: role 0 = GEMM engine, 1 = recurrence, 2 = output engine, 3 = beam search.  Plain non-blocking streams unless the
 // tunables search_cus / am_cus partition the chip (hostutil.cpp).
 void create_engine_stream(hipStream_t* st, int role, bool high_priority = false);
+int hw_queues();                          // hardware queues of this process: GPU_MAX_HW_QUEUES, or the runtime's own four where that is not set or no number (hostutil.cpp)
 unsigned long long layout_generation();   // bumped when any DevBuf / PinnedBuf moves or a tunable changes (hostutil.cpp): what a captured graph may have baked in
 void copy_h2d(void* dst_dev, const PinnedBuf& src, size_t bytes, hipStream_t st);
 void copy_d2h(PinnedBuf& dst, const void* src_dev, size_t bytes, hipStream_t st, size_t dst_offset = 0);

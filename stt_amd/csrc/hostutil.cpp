@@ -62,6 +62,12 @@ Tuning& tune() {
   return t;
 }
 
+int hw_queues() {
+  const char* e = getenv("GPU_MAX_HW_QUEUES");
+  const int n = e ? atoi(e) : 0;
+  return n > 0 ? n : 4;
+}
+
 // The searches take a compute unit's whole register file each (1024 lanes x 128 registers) for most of a batch; the acoustic engines
 // live on whatever is left.  Left to the dispatcher, who sits where is decided launch by launch.  With search_cus = N the search streams
 // are confined to the CUs of mask bits [0, N) and (am_cus) the chosen acoustic engines to the rest: a fixed partition.  (A masked stream

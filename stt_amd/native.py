@@ -71,6 +71,7 @@ STT_AMD_H = [
 STT_AMD_TEST_H = [      # include/stt_amd_test.h: libstt_test.so only
     "STTX_DebugBatchProbs", "STTX_TestLstmSteps", "STTX_TestDenseHybrid", "STTX_DebugSlowRows", "STTX_TestHybridChain", "STTX_TestDense",
     "STTX_TestMath", "STTX_TestLm", "STTX_TestDictionaryWalk", "STTX_DebugLimitArena", "STTX_TestFleetRecords", "STTX_DebugFleetFailShard",
+    "STTX_TestHwQueues",
 ]
 
 _lib = None
@@ -185,6 +186,7 @@ def lib():
         "STTX_DenseBlocksWorkspace": (C.c_ulonglong, [ci, ci, cl, cl, cl]),
         "STTX_TestFleetRecords": (pp(vp), [pp(cs), pp(cu), cu, cu]),
         "STTX_DebugFleetFailShard": (ci, [vp, ci]),
+        "STTX_TestHwQueues": (ci, []),
     }
     for name, (res, args) in sig.items():
         if name in STT_AMD_TEST_H and not TEST_HOOKS:

@@ -244,3 +244,18 @@ def test_bench_final_line_stays_short_enough_for_the_driver():
     # and main() prints it LAST, after the detail
     src = open(os.path.join(ROOT, "bench.py")).read()
     assert src.index('print("bench_detail: " + detail)') < src.index("print(json.dumps(compact_line(res)")
+
+
+def test_hardware_queues_of_a_process():
+    """What the engine places its streams by: GPU_MAX_HW_QUEUES, and the runtime's own four in a process that does not set it (a consumer that does not call
+    STTX_ConfigureRuntime), or not to a number above zero."""
+    from stt_amd import native
+    L, libc = native.lib(), C.CDLL(None)
+    libc.getenv.restype = C.c_char_p
+    before = libc.getenv(b"GPU_MAX_HW_QUEUES")
+    try:
+        for value, queues in ((None, 4), ("", 4), ("many", 4), ("0", 4), ("-3", 4), ("1", 1), ("4", 4), ("8", 8), ("16", 16)):
+            os.unsetenv("GPU_MAX_HW_QUEUES") if value is None else os.putenv("GPU_MAX_HW_QUEUES", value)
+            assert L.STTX_TestHwQueues() == queues, value
+    finally:
+        os.unsetenv("GPU_MAX_HW_QUEUES") if before is None else os.putenv("GPU_MAX_HW_QUEUES", before.decode())
