@@ -483,3 +483,51 @@ def test_block_tensors_whose_rows_are_refused():
                 call()
     with pytest.raises(ValueError, match="multiples of 16"):
         blocks.dense_blocks(x, blocks.BlockTensor(w.values, w.scale[:1].expand(3, 8), 600, 128))
+
+
+@pytest.mark.parametrize("k", [256, 300, 513, 1025, 2048])
+def test_dense_256_row_tiles_along_k(k):
+    """The tile of the largest products over two blocks along k and more, partial ones and several words of scale bytes; equal in every bit: sums of multiples of
+    2^-2 below 2^18 are exact in 32 bits."""
+    m, n = 4500, 4100
+    rng = np.random.default_rng(k)
+    x, xd = whole_blocks(rng, m, k, 1)
+    w, wd = whole_blocks(rng, n, k, 128)
+    bias = rng.integers(-900, 901, n) / 4.0
+    want = R.dense(xd, wd, bias, None)
+    bg = torch.from_numpy(bias).float().cuda()
+    for t, dt in TYPES.items():
+        np.testing.assert_array_equal(host(blocks.dense_blocks(x, w, bg, dtype=dt)), host(torch.from_numpy(want).float().to(dt)), err_msg=t)
+    check_blocks(blocks.dense_blocks(x, w, bg, relu_clip=100.0, dtype=E4M3), R.dense(xd, wd, bias, 100.0), 1)
+
+
+@pytest.mark.parametrize("kind", ["blocks", "f16"])
+def test_dense_256_row_tiles_real_values(kind):
+    """As test_dense_real_values (its tolerance), in the tile of the largest products."""
+    m, k, n = 4500, 2048, 4100
+    g = torch.Generator().manual_seed(6)
+    x = (torch.randn(m, k, generator=g) * torch.exp(torch.randn(m, 1, generator=g))).half()
+    w = torch.randn(n, k, generator=g) * torch.exp(torch.randn(n, 1, generator=g)) / k ** 0.5
+    bias = torch.randn(n, generator=g)
+    xd, wd = (R.values(*R.quantize(host(v), br), k, br) for v, br in ((x, 1), (w, 128)))
+    xin = gpu_blocks(*R.quantize(host(x), 1), k, 1) if kind == "blocks" else x.cuda()
+    want, size = R.dense(xd, wd, host(bias)), np.abs(xd) @ np.abs(wd).T + np.abs(host(bias))
+    got = host(blocks.dense_blocks(xin, blocks.quantize_blocks(w.cuda(), 128), bias.cuda(), dtype=torch.float32))
+    assert (np.abs(got - want) <= (k + 1) * 2.0 ** -23 * size * (1 + 2.0 ** -24) + 2.0 ** -24 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("k", [100, 494, 2048])
+def test_tiles_of_every_height_give_the_same_bits(k):
+    """Real rows in batches that take tiles of 32, 64, 128 and 256 rows, from the batch's start and from within a tile: a row's sums run in one order, so its f32
+    bits and its blocks are the same in all of them."""
+    n = 4100
+    x = torch.randn(4500, k, device="cuda") * torch.exp(torch.randn(4500, 1, device="cuda"))
+    xb = blocks.quantize_blocks(x)
+    w = blocks.quantize_blocks(torch.randn(n, k, device="cuda"), 128)
+    b = torch.randn(n, device="cuda")
+    whole, held = blocks.dense_blocks(xb, w, b, dtype=torch.float32), blocks.dense_blocks(xb, w, b, relu_clip=20.0, dtype=E4M3)
+    for first, rows in ((0, 200), (37, 224), (0, 600), (101, 896), (0, 2000), (333, 3800)):
+        part = blocks.BlockTensor(xb.values[first:first + rows], xb.scale[first:first + rows], k)
+        assert torch.equal(blocks.dense_blocks(part, w, b, dtype=torch.float32).view(torch.int32), whole[first:first + rows].view(torch.int32)), (first, rows)
+        h = blocks.dense_blocks(part, w, b, relu_clip=20.0, dtype=E4M3)
+        assert torch.equal(h.values.view(torch.uint8), held.values[first:first + rows].view(torch.uint8)) and torch.equal(h.scale, held.scale[first:first + rows]), (first, rows)

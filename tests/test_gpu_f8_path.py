@@ -133,3 +133,16 @@ def test_off_by_default(tmp_path):
     finally:
         native.set_tuning("am_f8", 0)
     assert f8.acousticMode() == 2 and not np.array_equal(f8.acousticProbs([a])[0], before)
+
+
+def test_wide_batches_give_an_utterance_its_own_bits(tmp_path):
+    """2048 units: an utterance alone (250 rows: tiles of 32 rows, of 64 in the x half of the cell), among eight (2000 rows: 64, 256), among twenty-four (6000: 128,
+    256) and among forty (10000: 256) gets the same probabilities in every bit."""
+    m = _model(tmp_path, synth.synth_weights(34, n_hidden=2048), "wide2")
+    audio = [synth.synth_audio(80000, seed=900 + i) for i in range(40)]
+    batches = [m.acousticProbs(audio[:n]) for n in (8, 24, 40)]
+    for i in (0, 3, 7, 20, 39):
+        alone = m.acousticProbs([audio[i]])[0]
+        assert alone.shape[0] == 250
+        for among in batches:
+            assert i >= len(among) or np.array_equal(alone, among[i]), (i, len(among))
