@@ -651,10 +651,9 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
       }
     }
   };
-  if constexpr (AHEAD > 2) last(std::integral_constant<int, 3>());
   if constexpr (AHEAD > 1) last(std::integral_constant<int, 2>());
   last(std::integral_constant<int, 1>());
-  static_assert((STAGES - 1) % SUB == 0 && AHEAD <= 3, "whole blocks in flight, and scale words of two groups of four");
+  static_assert((STAGES - 1) % SUB == 0 && AHEAD <= 2, "whole blocks in flight, and scale words of two groups of four");
 #undef BLOCKS_ARRIVE
   if (a.y_type != BLOCKS_F32) __syncthreads();      // every wave is done reading the stages: LDS is the results' now
   const int64_t mw = m0 + wm * MJ * 16;
