@@ -91,17 +91,20 @@ def _bad_blocks(b, what, block_rows):
 
 
 def _blocks(b, what, block_rows):
-    """(rows, cols, values' address and row stride, scales' address and row stride, device index); block_rows: the ones that may be.  The stride of a single row,
-    which torch leaves open, is the width."""
+    """(rows, cols, values' address and row stride, scales' address and row stride, device index); block_rows: the ones that may be"""
     v, s, cols, br = b.values, b.scale, b.cols, b.block_rows
     vs, ss = v.shape, s.shape
-    if (v.dtype is not E4M3 or s.dtype is not _UINT8 or len(vs) != 2 or len(ss) != 2 or br not in block_rows or cols < 1 or vs[1] < -(-cols // BLOCK) * BLOCK or
-            ss[0] * br < vs[0] or ss[1] < -(-cols // 512) * 4 or not v.is_cuda or v.get_device() != s.get_device() or v.stride(1) != 1 or s.stride(1) != 1):
+    if (v.dtype is not E4M3 or s.dtype is not _UINT8 or len(vs) != 2 or len(ss) != 2 or br not in block_rows or cols < 1 or vs[1] < (wide := -(-cols // BLOCK) * BLOCK) or
+            ss[0] * br < vs[0] or ss[1] < (words := -(-cols // 512) * 4) or not v.is_cuda or v.get_device() != s.get_device()):
         raise _bad_blocks(b, what, block_rows)
-    wide, words = -(-cols // BLOCK) * BLOCK, -(-cols // 512) * 4
-    ldq, lds, q, scale = v.stride(0) if vs[0] > 1 else wide, s.stride(0) if ss[0] > 1 else words, v.data_ptr(), s.data_ptr()
-    if ldq < wide or lds < words or (ldq | q) & 15 or (lds | scale) & 3:
-        raise _bad_blocks(b, what, block_rows)
+    (ldq, one), (lds, unit), q, scale = v.stride(), s.stride(), v.data_ptr(), s.data_ptr()
+    if one != 1 or unit != 1 or ldq < wide or lds < words or (ldq | q) & 15 or (lds | scale) & 3:
+        if vs[0] < 2:                       # (torch leaves the stride of a single row open)
+            ldq = wide
+        if ss[0] < 2:
+            lds = words
+        if one != 1 or unit != 1 or ldq < wide or lds < words or (ldq | q) & 15 or (lds | scale) & 3:
+            raise _bad_blocks(b, what, block_rows)
     return vs[0], cols, q, ldq, scale, lds, v.get_device()
 
 
