@@ -13,8 +13,8 @@
 // without rounding (4 significand bits, an 8-bit exponent), so the scales cost no arithmetic of their own and the sums of all blocks stay in one f32
 // accumulator.  The 8-bit matrix instructions (v_mfma_scale_f32_16x16x128_f8f6f4, v_mfma_f32_16x16x32_fp8_fp8) would be twice as fast, but do not
 // keep 32 bits: products far below the largest ones they are added to lose bits.  Measured over 2048 products of values of all magnitudes, error
-// relative to the result: 5e-5 on either of them, 3e-7 on the bf16 form; on layer outputs 1e-5 against 4e-8, which four layers in blocks
-// one behind the other turn into 1.5 % of the result.
+// relative to the result: 5e-5 on either of them, 3e-7 on the bf16 form; clipped activations by normal weights 1e-5 against 4e-8
+// (benchmarks/blocks_sums_probe.hip, profiles/blocks_sums.txt), which four layers in blocks one behind the other turned into 1.5 % of the result.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -126,7 +126,7 @@ __device__ __forceinline__ unsigned pack4_(float a, float b, float c, float d, f
 
 // ------------------------------------------------------------------------------------------- rows of 1 x 128
 // A wave per four blocks of a row (one word of scale bytes), sixteen lanes a block, eight values a lane: one pass, 16 bytes a lane and load for 16-bit rows.
-// HBM bounds it: 32000 x 2048 f16 in 37.8 us, 5.2 TB/s of what it reads and writes (a copy of 1 GiB: 5.1); f32 the same rate.
+// HBM bounds it: 32000 x 2048 f16 in 37.7 us, 5.2 TB/s of what it reads and writes (a copy of 1 GiB: 5.1); f32, the same matrix each time, 55.3 us, 5.9.
 template <int T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(BlocksQuantArgs a) {
   const int lane = threadIdx.x & 63;
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(BlocksQuantArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------- tiles of 128 x 128
-// A workgroup per tile, the tile in registers between the search for its largest value and the conversion.  HBM: 8192 x 2048 f32 in 15.2 us, 5.5 TB/s.
+// A workgroup per tile, the tile in registers between the search for its largest value and the conversion.  HBM: 8192 x 2048 f32 in 15.2 us, 5.5 TB/s; f16 9.9 us, 5.1.
 template <int T>
 __global__ __launch_bounds__(256) void quantize_tiles_kernel(BlocksQuantArgs a) {
   __shared__ unsigned s_top[2][4];
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256) void quantize_tiles_kernel(BlocksQuantArgs a) 
 }
 
 // ------------------------------------------------------------------------------------------- the way back
-// As the rows kernel, the other way.  HBM: 32000 x 2048 to bf16 in 37.5 us, 5.3 TB/s.
+// As the rows kernel, the other way.  HBM: 32000 x 2048 to bf16 in 37.5 us, 5.3 TB/s, to f32 60, 5.4; 8192 x 2048 in tiles to f16 9.8, 5.1.
 template <int T>
 __global__ __launch_bounds__(256) void dequantize_kernel(BlocksDequantArgs a) {
   const int lane = threadIdx.x & 63;
@@ -301,9 +301,9 @@ template <> struct XQuarter<BLOCKS_E4M3> {
 
 // Few rows: 16 output features by 16 MT rows per workgroup, the blocks along k dealt to its eight waves; operands straight from L2 / HBM into
 // registers, the waves' sums meet in LDS (in the order of the waves: the same bits every time).  What bounds it is how much a compute unit takes in,
-// some 30 GB/s of its part of w and of all of x: sixteen features a workgroup put 2048 of them on 128 units (16 rows, k = 2048: 4.1 us of which a
-// launch is 2; asking for two or four blocks ahead changes nothing), and a block of 128 features a workgroup, which could write y in blocks itself,
-// is on 16 units and takes 18.7 us.
+// some 30 GB/s of its part of w and of all of x: sixteen features a workgroup put 2048 of them on 128 of the 256 units (16 rows, k = 2048: 4.4 us, of which
+// a launch is 2 and 64 KB a workgroup the rest; asking for two or four blocks ahead changed nothing).  A block of 128 features a workgroup, which could
+// write y in blocks itself, is on 16 units and took 18.7 us; other numbers of features have not been tried.
 template <int T, int MT>
 __global__ __launch_bounds__(512) void dense_few_kernel(BlocksDenseArgs a) {
   constexpr int KW = 8;
@@ -368,8 +368,8 @@ __global__ __launch_bounds__(512) void dense_few_kernel(BlocksDenseArgs a) {
 }
 
 // Sixteen rows of a wave's results in 8 or 16 bits through LDS (its own part of it), so that they leave 16 bytes a lane along a row: straight from the
-// accumulators a store writes an eighth to a quarter of a line in each of sixteen rows.  Measured, us straight | through LDS: 6144 x 2048 features in blocks
-// 53.1 | 49.9, 6144 x 8192 f16 174 | 171; f32, half a line a row and store, is better off straight (2048 x 8192 61.2 | 65.8).
+// accumulators a store writes an eighth to a quarter of a line in each of sixteen rows.  Measured when it came, us straight | through LDS: 6144 x 2048 features in
+// blocks 55.4 | 52.6, 6144 x 8192 f16 189 | 173; f32, half a line a row and store, is better off straight (2048 x 8192 61.2 | 65.8).
 // Lane (li, g) holds 4 values = `Q` bytes at feature 16 i + 4 g of row li.
 template <int NI, int Q> struct RowsOut {
   static constexpr int BYTES = NI * 4 * Q, PITCH = BYTES + 16, CHUNKS = BYTES / 16;      // of a row; the pitch keeps a column's rows on different banks
@@ -503,11 +503,11 @@ __device__ __forceinline__ void tile_results_as_(const BlocksDenseArgs& a, f32x4
 // bf16; the scale words of four blocks along k go the same way.  The 16-byte chunks of a staged row are permuted so that the sixteen lanes a ds_read_b128 is
 // serviced in are on different banks: chunk c of a 64-byte row r at slot c ^ (row bit 3) * 2, of a 128-byte row at c ^ (r / 2 mod 8).
 // Large tiles: a wave of the 256-row tile turns 12 fragments into bf16 for 64 products a step of 64 (96 conversions, which the other workgroup's
-// products hide); two such workgroups fit a compute unit, three of the 128-row tile.  32000 x 8192 x 2048 to f32: 914 us = 1175 TFLOP/s, the matrix cores
-// busy 56 % of the time; a library's bf16 product of that shape takes 919 us and writes half as much.  The clock falls with the data (the same
+// products hide); two such workgroups fit a compute unit, three of the 128-row tile.  32000 x 8192 x 2048 to f32: 870 - 890 us by the card, 1234 - 1206 TFLOP/s, the matrix
+// cores busy 58 % of the time; a library's bf16 product of that shape takes 919 us and writes half as much.  The clock falls with the data (the same
 // call on operands of all ones: 13 % less): power, not one unit, is what is left.
 // Small tiles: one wave a SIMD unit, so a step's latencies -- barrier, LDS, conversion, product -- add up, and more stages in flight change nothing (64
-// rows, 64 values a step, 3 / 5 / 7 stages: 15.6 / 15.1 / 15.0 us at k = 2048): 128 values a step halve the barriers (14.4) and 32 rows the work (11.3).
+// rows, 64 values a step, 3 / 5 / 7 stages: 15.6 / 15.1 / 15.0 us at k = 2048): 128 values a step halve the barriers (14.5) and 32 rows the work (10.6).
 template <int BM, int WN, int STAGES, int KS>
 __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
   constexpr int BN = 128, WM = 4 / WN, NI = 8 / WN, MJ = BM / 16 / WM;
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256, 2) void dense_tile_kernel(BlocksDenseArgs a) {
   int tile_n;
   int64_t tile_m;
   {  // workgroup i runs on XCD i % 8: every XCD takes a run of tiles, 1024 rows at a time over all features, so that what it works on at once shares rows and
-     // features (32000 x 8192 x 2048: 995 us with 1024 rows, 1009 and 1038 with 512 and 2048)
+     // features (32000 x 8192 x 2048: 868 us with 1024 rows, 867 and 902 with 512 and 2048)
     constexpr unsigned GM = 1024 / BM;      // (less than 2^24 tiles: checked on the host)
     const unsigned tn = (unsigned)tiles_n, tiles_m = (unsigned)((a.M + BM - 1) / BM), total = tn * tiles_m, per = (total + 7) / 8;
     const unsigned idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -679,11 +679,13 @@ template <int T, int MT>
 void few_(const BlocksDenseArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((dense_few_kernel<T, MT>), dim3((a.N + 15) / 16, (unsigned)((a.M + 16 * MT - 1) / (16 * MT))), dim3(512), 0, st, a);
 }
-// Tiles of 16 rows per workgroup of the few-rows form, 0 where the tiled form is taken.  The former costs what its workgroups cost -- some 4.2 us up to 256 of
-// them, then in proportion -- and more rows a workgroup read the weights fewer times; the latter takes 11.3 us at k = 2048 for the latency of its steps,
+// Tiles of 16 rows per workgroup of the few-rows form, 0 where the tiled form is taken.  The former costs what its workgroups cost -- some 4.4 us up to 256 of
+// them, then in proportion -- and more rows a workgroup read the weights fewer times; the latter takes 10.5 us at k = 2048 for the latency of its steps,
 // but does more work in a given time.  So: the fewest rows that need at most 256 workgroups, or up to 32 rows where those need at most 512.
-// Measured at k = 2048, us for 1, 2, 4 tiles a workgroup | tiled: 64 x 2048 features 6.3, 5.5, 7.7 | 11.4; 16 x 8192 6.1, 6.8, 8.2 | 11.3;
-// 32 x 8192 10.2, 8.5, 9.9 | 11.3; 64 x 8192 18.3, 14.9, 13.2 | 11.7; 128 x 2048 10.3, 8.5, 7.9 | 11.5; 256 x 2048 18.4, 15.0, 13.2 | 11.6.
+// Measured at k = 2048, us for 1, 2, 4 tiles a workgroup | tiled: 64 x 2048 features 6.6, 5.7, 7.8 | 10.6; 16 x 8192 6.5, 7.3, 8.6 | 10.5;
+// 32 x 8192 10.6, 8.9, 10.3 | 10.6; 64 x 8192 18.9, 15.2, 13.5 | 10.9; 128 x 2048 10.8, 9.0, 8.2 | 10.6; 256 x 2048 19.2, 15.5, 13.6 | 10.8.
+// Both parts of the work grow with k, so k is not asked for: at 128, 494 and 4096 the choice is within a tenth of the best (profiles/blocks_forms.txt) but for
+// 128 x 2048 at k = 128 (3.8 | 3.2 with one tile) and the border of 29 features, 6144 rows: 9.7 | 8.8 with one tile, 24 | 17 at k = 4096.
 int few_tiles_(int64_t M, int N) {
   const int64_t n = (N + 15) / 16;
   for (int mt = 1; mt <= 4; mt *= 2) {
@@ -693,11 +695,11 @@ int few_tiles_(int64_t M, int N) {
   return 0;
 }
 
-// Rows of a tile: larger tiles do more work for what they stage, smaller ones fill the chip sooner.  Measured at k = 2048, us for 32 / 64 / 128 / 256 rows:
-// 512 x 2048 features 12.2 / 14.7 / 23.2 / 33.7 and 1024 x 2048 15.8 / 15.8 / 23.8 / 34.2 (256 and 512 tiles of 32 rows); 512 x 8192 29.1 / 23.1 / 26.3 /
-// 35.9 and 2048 x 2048 27.2 / 21.8 / 25.1 / 35.7 (256 tiles of 128 rows); 1024 x 8192 51.5 / 40.9 / 37.8 / 38.3 and 6144 x 2048 in blocks
-// 74.7 / 55.3 / 49.5 / 55.8 (256 and 384 tiles of 256 rows: less than two workgroups for every compute unit); 2048 x 8192 98 / 77 / 69 / 63;
-// 6144 x 8192 f16 280 / 217 / 179 / 162.
+// Rows of a tile: larger tiles do more work for what they stage, smaller ones fill the chip sooner.  Measured at k = 2048, f32 results, us for 32 / 64 / 128 / 256 rows:
+// 512 x 2048 features 11.3 / 14.9 / 23.4 / 33.4 and 1024 x 2048 16.3 / 16.3 / 23.9 / 33.9 (256 and 512 tiles of 32 rows); 512 x 8192 28.9 / 22.7 / 25.9 /
+// 35.4 and 2048 x 2048 30.0 / 23.5 / 27.0 / 35.6 (256 tiles of 128 rows); 1024 x 8192 53.8 / 40.1 / 36.2 / 36.6 and 6144 x 2048 74.2 / 55.9 / 50.4 /
+// 54.1 (256 and 384 tiles of 256 rows: less than two workgroups for every compute unit); 2048 x 8192 97 / 75 / 65 / 59; 6144 x 8192 285 / 223 / 188 / 171.
+// At k = 128, 494 and 4096 the choice is within a tenth of the best too (profiles/blocks_forms.txt).
 int tile_rows_(int64_t M, int N) {
   const int64_t tiles_n = ((int64_t)N + 127) / 128;
   if (tiles_n * ((M + 31) / 32) <= 256) return 32;
@@ -761,8 +763,10 @@ struct Plan {
   bool fused = false;                  // x is quantised by the few-rows form on the way: once for every 16 features
   int64_t ldq = 0, lds = 0, ldy = 0;   // of x in blocks, of y in f32
   size_t x_bytes = 0, y_bytes = 0;
-  // Quantising on the way saves a launch (some 3 us) and costs in proportion to rows x features / 16.  Measured, us on the way | first, k = 2048:
-  // 16 x 2048 5.8 | 7.1; 1009 x 29 5.7 | 7; 64 x 2048 f16 9.6 | 8.1; 4000 x 29 f32 18.4 | 15.4: up to 256 workgroups of 16 rows.
+  // Quantising on the way saves a launch (some 2 us) and costs in proportion to rows x features / 16: up to 256 workgroups of 16 rows.  Measured, us on the
+  // way | first, f16, k = 2048: 16 x 2048 5.8 | 6.7; 32 x 2048 6.1 | 6.8; 64 x 2048 10.5 | 8.0; 1009 x 29 5.7 | 8.1; 2048 x 29 6.0 | 10.3; 4000 x 29 9.3 |
+  // 14.8; f32, twice the bytes: 16 x 2048 7.2 | 6.7; 64 x 2048 12.1 | 8.1; 1009 x 29 7.7 | 8.3; 2048 x 29 11.9 | 10.3; 4000 x 29 19.8 | 14.5.  The border moves
+  // with k: at 128 it would lie higher (64 x 2048 3.5 | 5.1), for f32 rows at 4096 lower (16 x 2048 11.7 | 9.1) -- profiles/blocks_forms.txt.
   Plan(int x_type, int y_type, int64_t M, int N, int K, int ordered) {
     mt = ordered ? 0 : few_tiles_(M, N);
     fused = x_type != BLOCKS_E4M3 && mt == 1 && (M + 15) / 16 * ((N + 15) / 16) <= 256;
