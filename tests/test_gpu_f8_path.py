@@ -146,3 +146,48 @@ def test_wide_batches_give_an_utterance_its_own_bits(tmp_path):
         assert alone.shape[0] == 250
         for among in batches:
             assert i >= len(among) or np.array_equal(alone, among[i]), (i, len(among))
+
+
+@pytest.mark.parametrize("kw", [{}, {"quantize": True, "per_channel": True}, {"f16_weights": True}], ids=["f32", "int8", "f16"])
+def test_any_file_takes_it(tmp_path, kw):
+    """A `.tflite` export of either kind runs as the container of its (de-quantised) tensors does, also where am_i8 asks for the file's own arithmetic."""
+    from stt_amd import Model, modelfile, tflitefile
+    w = synth.synth_weights(35, n_hidden=256)
+    p, q = str(tmp_path / "m.tflite"), str(tmp_path / "m.sttw")
+    eff = tflitefile.write_tflite(p, w, synth.ENGLISH_LABELS, beam_width=64, **kw)
+    modelfile.write_model(q, {n: eff[n] for n in modelfile.TENSOR_ORDER}, synth.ENGLISH_LABELS, beam_width=64)
+    native.set_tuning("am_f8", 1), native.set_tuning("am_i8", 1)
+    try:
+        a, b = Model(p), Model(q)
+    finally:
+        native.set_tuning("am_f8", 0), native.set_tuning("am_i8", -1)
+    assert a.acousticMode() == b.acousticMode() == 2
+    audio = [synth.synth_audio(n, seed=60 + n) for n in (300, 9000, 31000)]
+    for x, y in zip(a.acousticProbs(audio), b.acousticProbs(audio)):
+        assert np.array_equal(x, y)
+    assert a.sttBatch(audio) == b.sttBatch(audio)
+
+
+def test_streams_advanced_together(small):
+    """Streams that join and end at different hops, advanced by one call a hop for all of them (their passes replayed from graphs), end with what each is alone."""
+    from stt_amd import model as M
+    m, _ = small
+    audio = [synth.synth_audio(int(n), seed=2500 + i) for i, n in enumerate((40000, 5120, 23000, 61000, 300, 17000))]
+    want = [m.stt(a) for a in audio]
+    assert any(want)
+    for turn in range(2):
+        live, got, k = [], {}, 0
+        while k < len(audio) or live:
+            if k < len(audio):
+                live.append([k, m.createStream(), 0])
+                k += 1
+            M.feedAudioContentBatch([s for _, s, _ in live], [audio[i][at:at + 5120] for i, _, at in live])
+            M.intermediateDecodeBatch([s for _, s, _ in live])
+            for stream in live:
+                stream[2] += 5120
+            ended = [e for e in live if e[2] >= len(audio[e[0]])]
+            if ended:
+                for (i, _, _), text in zip(ended, M.finishStreamBatch([s for _, s, _ in ended])):
+                    got[i] = text
+                live = [e for e in live if e[2] < len(audio[e[0]])]
+        assert [got[i] for i in range(len(audio))] == want, turn
