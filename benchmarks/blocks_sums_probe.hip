@@ -1,6 +1,6 @@
 // Which matrix instruction keeps 32 bits in a sum of e4m3 products: the two 8-bit ones against e4m3 values taken as bf16 (exact), one wave, 16 x 16 sums over
 // k values, against the same sums in 64 bits.  Error relative to the results (root of summed squares).
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 blocks_sums_probe.hip -o /tmp/blocks_sums_probe && /tmp/blocks_sums_probe
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops blocks_sums_probe.hip -o /tmp/blocks_sums_probe && /tmp/blocks_sums_probe
 #include <hip/hip_runtime.h>
 
 #include <cmath>
